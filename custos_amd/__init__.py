@@ -16,4 +16,4 @@ from .capi import (  # noqa: F401
     lib_path,
     load_library,
 )
-from .device import HIP, Buffer, Graph  # noqa: F401
+from .device import HIP, Buffer, Checkpoint8, Graph  # noqa: F401

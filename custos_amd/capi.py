@@ -79,6 +79,25 @@ class Tuning(C.Structure):
     ]
 
 
+class GroupNormDesc(C.Structure):
+    """custos_hip_group_norm_desc"""
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("param_dtype", C.c_int32),
+        ("activation", C.c_int32),
+        ("flags", C.c_int32),
+        ("samples", C.c_uint64),
+        ("positions", C.c_uint64),
+        ("channels", C.c_uint64),
+        ("groups", C.c_uint64),
+        ("eps", C.c_double),
+    ]
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+GRAD_OVERWRITE = 1
+
+
 def lib_path() -> str:
     return os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libcustos_hip.so")
 
@@ -168,6 +187,8 @@ PROTOTYPES = {
     "custos_hip_set_graph_verify": (C.c_int32, [_P, C.c_int32]),
     "custos_hip_graph_edge_count": (C.c_int32, [_P, C.POINTER(C.c_size_t)]),
     "custos_hip_graph_destroy": (C.c_int32, [_P, _P]),
+    "custos_hip_group_norm": (C.c_int32, [_P, C.POINTER(GroupNormDesc)] + [C.c_uint64] * 7),
+    "custos_hip_add_group_norm_grad": (C.c_int32, [_P, C.POINTER(GroupNormDesc)] + [C.c_uint64] * 13),
     "custos_hip_timer_begin": (C.c_int32, [_P]),
     "custos_hip_timer_end": (C.c_int32, [_P, C.POINTER(C.c_double)]),
     "custos_hip_timer_mark": (C.c_int32, [_P, C.c_uint32]),

@@ -698,6 +698,12 @@ int32_t lower_node(custos_hip_device* dev, const std::vector<RecNode>& nodes, co
         ln.grid = dim3(first.grid3[0], first.grid3[1], first.grid3[2]);
         ln.block = dim3(first.block3[0], first.block3[1], first.block3[2]);
         ln.shared_mem = first.shared_mem;
+    } else if (first.type == RecNode::Op) {
+        ln.args = first.arg_values;
+        ln.func = first.op_func;
+        ln.module_fn = first.op_module_fn;
+        ln.grid = dim3(first.grid3[0], first.grid3[1], first.grid3[2]);
+        ln.block = dim3(first.block3[0], first.block3[1], first.block3[2]);
     } else if (first.type == RecNode::Fill) {
         const unsigned long long a0 = first.bytes, a1 = first.head, a2 = first.n_vec;
         ln.args = {value(&first.ptrs[0], 8), value(&a0, 8), value(&a1, 8), value(&a2, 8)};
@@ -773,7 +779,9 @@ std::vector<uint64_t> signature(const std::vector<RecNode>& nodes) {
         sig.insert(sig.end(), n.ptrs.begin(), n.ptrs.end());
         sig.push_back(n.pattern.size());
         sig.insert(sig.end(), n.pattern.begin(), n.pattern.end());
-        if (n.type != RecNode::Source) continue;
+        if (n.type != RecNode::Source && n.type != RecNode::Op) continue;
+        sig.push_back(reinterpret_cast<uint64_t>(n.op_func));
+        // (what an operator's launch reads and writes follows from its arguments)
         for (int d = 0; d < 3; d++) sig.push_back(static_cast<uint64_t>(n.grid3[d]) << 32 | n.block3[d]);
         sig.push_back(n.shared_mem);
         sig.push_back(n.arg_values.size());
@@ -1151,6 +1159,7 @@ int32_t build_graph(custos_hip_device* dev, custos_hip_graph* g) {
                 const RecNode& first = nodes[p.members[0]];
                 if (first.type == RecNode::Fill) g->node_names.push_back(first.pattern.empty() ? "custos_fill_zero" : "custos_fill_pattern");
                 else if (first.type == RecNode::Source) g->node_names.push_back(first.k->spec.name);
+                else if (first.type == RecNode::Op) g->node_names.push_back(first.op_name);
                 else g->node_names.push_back(p.kern->spec.name + (p.members.size() == 1 ? "" : p.ragged ? "_ragged" : "_batched"));
             }
             lowered[level].push_back(std::move(ln));

@@ -251,6 +251,116 @@ ResolvedShape shape_of_launch(custos_hip_device* dev, const custos_hip_kernel* k
     return shape;
 }
 
+// ---- operators ----
+
+int32_t launch_op(custos_hip_device* dev, const OpLaunch& op) {
+    if (dev->capturing) {
+        if (dev->matching && dev->matched < dev->previous_recorded.size()) {
+            const RecNode& was = dev->previous_recorded[dev->matched];
+            bool same = was.type == RecNode::Op && was.op_func == op.func && was.arg_values.size() == op.n_args &&
+                        was.acc.size() == op.n_acc && was.grid3[0] == op.grid.x && was.grid3[1] == op.grid.y &&
+                        was.block3[0] == op.block.x;
+            for (size_t i = 0; same && i < op.n_args; i++)
+                same = was.arg_values[i].size() == op.args[i].bytes &&
+                       std::memcmp(was.arg_values[i].data(), op.args[i].value, op.args[i].bytes) == 0;
+            for (size_t i = 0; same && i < op.n_acc; i++)
+                same = was.acc[i].begin == op.acc[i].begin && was.acc[i].end == op.acc[i].end && was.acc[i].write == op.acc[i].write;
+            if (same) {
+                dev->matched++;
+                return CUSTOS_HIP_OK;
+            }
+        }
+        stop_matching(dev);
+        RecNode node;
+        node.type = RecNode::Op;
+        node.k = op.kernel;
+        node.op_func = op.func;
+        node.op_module_fn = op.module_fn;
+        node.op_name = op.name;
+        node.grid3[0] = op.grid.x, node.grid3[1] = op.grid.y, node.grid3[2] = 1;
+        node.block3[0] = op.block.x, node.block3[1] = 1, node.block3[2] = 1;
+        for (size_t i = 0; i < op.n_args; i++) {
+            const unsigned char* p = static_cast<const unsigned char*>(op.args[i].value);
+            node.arg_values.emplace_back(p, p + op.args[i].bytes);
+        }
+        node.acc.assign(op.acc, op.acc + op.n_acc);
+        dev->recorded.push_back(std::move(node));
+        return CUSTOS_HIP_OK;
+    }
+    // (the launch shapes of generated kernels follow what ran before them, operators included)
+    unsigned long long touched = 0;
+    for (size_t i = 0; i < op.n_acc; i++) touched += op.acc[i].end - op.acc[i].begin;
+    if (touched > kTrafficBeyondBytes) dev->recent.record(std::vector<Access>(op.acc, op.acc + op.n_acc));
+    void* args[16];
+    for (size_t i = 0; i < op.n_args; i++) args[i] = const_cast<void*>(op.args[i].value);
+    dev->launches_since_wait = true;
+    if (op.module_fn)
+        HIP_TRY(dev, hipModuleLaunchKernel(static_cast<hipFunction_t>(op.func), op.grid.x, op.grid.y, 1, op.block.x, 1, 1, 0,
+                                           dev->stream, args, nullptr));
+    else
+        HIP_TRY(dev, hipLaunchKernel(op.func, op.grid, op.block, args, 0, dev->stream));
+    return CUSTOS_HIP_OK;
+}
+
+int32_t operator_workspace(custos_hip_device* dev, size_t bytes, uint64_t* address) {
+    if (bytes > dev->workspace_bytes) {
+        size_t grown = std::max<size_t>(1u << 20, dev->workspace_bytes * 2);
+        while (grown < bytes) grown *= 2;
+        uint64_t fresh = 0;
+        int32_t rc = custos_hip_alloc(dev, grown, CUSTOS_HIP_ALLOC_UNINIT, &fresh);
+        if (rc != CUSTOS_HIP_OK) return rc;
+        // A graph, or the recording under way, may name the old area: it stays until the device goes
+        // (each is at least twice the one before, so together they are smaller than the last).
+        if (dev->workspace && dev->graphs.empty() && !dev->capturing) {
+            rc = custos_hip_free(dev, dev->workspace);
+            if (rc != CUSTOS_HIP_OK) {
+                (void)custos_hip_free(dev, fresh);
+                return rc;
+            }
+        }
+        dev->workspace = fresh;
+        dev->workspace_bytes = grown;
+    }
+    *address = dev->workspace;
+    return CUSTOS_HIP_OK;
+}
+
+int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* ops, size_t n, bool may_alias) {
+    auto refuse = [&](int32_t code, const Operand& o, const char* why) {
+        return set_error(dev, code, std::string(what) + ": " + o.name + " " + why);
+    };
+    for (size_t i = 0; i < n; i++) {
+        const Operand& o = ops[i];
+        if (o.ptr == 0) return refuse(CUSTOS_HIP_ERR_INVALID_ARGUMENT, o, "is a null address");
+        if (o.ptr % o.element) return refuse(CUSTOS_HIP_ERR_INVALID_ARGUMENT, o, "is not aligned to its element size");
+        if (o.rows > 1 && o.pitch_bytes < o.row_bytes) return refuse(CUSTOS_HIP_ERR_INVALID_ARGUMENT, o, "has a pitch shorter than its rows");
+        // (sizes of up to 2^56 bytes: no product here wraps)
+        if (o.rows > (1ull << 40) || o.pitch_bytes > (1ull << 40) || o.row_bytes > (1ull << 40) ||
+            static_cast<double>(o.rows) * static_cast<double>(std::max(o.pitch_bytes, o.row_bytes)) > 7e16)
+            return refuse(CUSTOS_HIP_ERR_TOO_LARGE, o, "is larger than any memory");
+        if (o.ptr > UINT64_MAX - (o.end() - o.ptr)) return refuse(CUSTOS_HIP_ERR_INVALID_ARGUMENT, o, "wraps around the address space");
+    }
+    for (size_t i = 0; i < n; i++) {
+        const Operand& w = ops[i];
+        if (!w.written) continue;
+        for (size_t j = 0; j < n; j++) {
+            const Operand& o = ops[j];
+            if (i == j || (o.written && j < i)) continue;
+            if (!(w.ptr < o.end() && o.ptr < w.end())) continue;
+            const bool one_pitch = w.pitch_bytes == o.pitch_bytes;
+            if (may_alias && !o.written && w.ptr == o.ptr && one_pitch && w.rows == o.rows && w.row_bytes == o.row_bytes) continue;
+            // slices of one wider tensor that share no element
+            if (one_pitch && w.rows > 1 && o.rows > 1) {
+                const uint64_t pitch = w.pitch_bytes;
+                const uint64_t ahead = w.ptr <= o.ptr ? (o.ptr - w.ptr) % pitch : (pitch - (w.ptr - o.ptr) % pitch) % pitch;
+                if (ahead >= w.row_bytes && ahead + o.row_bytes <= pitch) continue;
+            }
+            return set_error(dev, CUSTOS_HIP_ERR_BAD_OVERLAP, std::string(what) + ": " + w.name + " overlaps " + o.name);
+        }
+    }
+    return CUSTOS_HIP_OK;
+}
+
 }  // namespace custos_hip
 
 using namespace custos_hip;

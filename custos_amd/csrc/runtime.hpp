@@ -94,7 +94,7 @@ struct custos_hip_graph {
 
 // One recorded piece of work (while the device is recording, nothing is launched).
 struct RecNode {
-    enum Type { Kernel, Fill, Copy, Source } type = Kernel;
+    enum Type { Kernel, Fill, Copy, Source, Op } type = Kernel;
     custos_hip_kernel* k = nullptr;
     std::vector<uint64_t> ptrs;  // kernel: operand addresses in parameter order; fill: {ptr}; copy: {dst, src}
     unsigned long long n = 0, head = 0, n_vec = 0, bytes = 0;
@@ -108,6 +108,11 @@ struct RecNode {
     // reads and writes is unknown, so it orders itself against everything.
     unsigned int grid3[3] = {1, 1, 1}, block3[3] = {1, 1, 1}, shared_mem = 0;
     std::vector<std::vector<unsigned char>> arg_values;
+    // Op: a kernel of one of the library's operators, with the launch shape and argument values above; what
+    // it reads and writes is known (`acc`).
+    void* op_func = nullptr;     // hipFunction_t of a module, or the host handle of a library kernel
+    bool op_module_fn = false;
+    const char* op_name = "";    // what a profiler lists; lives as long as the device handle
 };
 
 // The address ranges of the last few launches, from which a launch learns whether it reads
@@ -268,6 +273,11 @@ struct custos_hip_device {
     std::unordered_map<std::string, custos_hip_kernel*> by_text;
     uint64_t compile_epoch = 0;  // advanced by every setting that changes what a text compiles to (tuning, eq and literal policy)
     std::vector<custos_hip_graph*> graphs;
+    // Work area of the operators that need one (operator_workspace): grown when an operator asks for
+    // more, shared by all of them -- the launches of a handle follow each other on its one stream, and
+    // a recorded launch names the part it uses among the ranges it writes.
+    uint64_t workspace = 0;
+    size_t workspace_bytes = 0;
 };
 
 namespace custos_hip {
@@ -387,6 +397,44 @@ int32_t launch_or_record(custos_hip_device* dev, custos_hip_kernel* k, const std
 // Workgroups of a single launch of `k` over n_vec vectors and n elements in the given shape.
 unsigned int launch_grid(const custos_hip_device* dev, const custos_hip_kernel* k, unsigned long long n,
                          unsigned long long n_vec, const ResolvedShape& shape);
+
+// An argument of an operator's kernel: where its value is and how long it is.
+struct OpArg {
+    const void* value;
+    size_t bytes;
+};
+// One launch of an operator's kernel, issued on the compute stream or recorded.  `acc`: every range it
+// reads or writes (one that is read and written is listed as written).
+struct OpLaunch {
+    const char* name;
+    void* func;              // host handle of a library kernel, or the hipFunction_t of a module
+    bool module_fn = false;
+    custos_hip_kernel* kernel = nullptr;  // of a generated kernel
+    dim3 grid, block;
+    const OpArg* args;
+    size_t n_args;
+    const Access* acc;
+    size_t n_acc;
+};
+int32_t launch_op(custos_hip_device* dev, const OpLaunch& op);
+// Work area of at least `bytes` bytes for launches issued or recorded now, 256-byte aligned.
+int32_t operator_workspace(custos_hip_device* dev, size_t bytes, uint64_t* address);
+
+// An operand of an operator: `rows` rows of `row_bytes` bytes that start `pitch_bytes` apart.
+struct Operand {
+    const char* name;
+    uint64_t ptr;
+    uint64_t rows, row_bytes, pitch_bytes;
+    bool written;
+    size_t element;  // bytes its address has to be a multiple of
+    uint64_t end() const { return rows == 0 || row_bytes == 0 ? ptr : ptr + (rows - 1) * pitch_bytes + row_bytes; }
+    Access access() const { return {ptr, end(), written}; }
+};
+// The checks every operator makes of its operands before it launches anything: no null or unaligned
+// address, no range that wraps, rows that do not overlap each other, and nothing written that another
+// operand covers -- except the same operand exactly (`may_alias`: the operator reads an element before it
+// writes it), and rows of one pitch that lie side by side (two slices of the same wider tensor).
+int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* ops, size_t n, bool may_alias);
 
 // graph.cpp
 int32_t replay_graph(custos_hip_device* dev, custos_hip_graph* g);

@@ -82,6 +82,52 @@ class Buffer:
             pass
 
 
+def _holds(name: str, buf: Buffer | None, length: int, dtype: str) -> None:
+    """An operator's operand has the element type the operator takes and is long enough."""
+    if buf is not None and (buf.dtype != dtype or buf.len < length):
+        raise ValueError(f"{name} is {buf.len} x {buf.dtype}, needs {length} x {dtype}")
+
+
+def _rows_len(rows: int, width: int, pitch: int) -> int:
+    """Elements from the first of `rows` rows of `width`, `pitch` apart, to the end of the last."""
+    return (rows - 1) * pitch + width if rows > 0 else 0
+
+
+def _group_norm_desc(dtype, gamma, beta, shape, groups, activation, eps, flags):
+    samples, positions, channels = shape
+    if activation not in capi.ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}")
+    params = gamma.dtype if gamma is not None else beta.dtype if beta is not None else "f32"
+    _holds("gamma", gamma, channels, params)
+    _holds("beta", beta, channels, params)
+    if min(samples, positions, channels, groups) < 0:
+        raise ValueError("negative size")
+    return capi.GroupNormDesc(capi.DTYPES[dtype][0], capi.DTYPES[params][0], capi.ACTIVATIONS[activation], flags, samples,
+                              positions, channels, groups, eps)
+
+
+class Checkpoint8:
+    """A buffer's values kept in 8 bits for the backward pass: a code per element, a scale per 128."""
+
+    BLOCK = 128
+
+    def __init__(self, device: "HIP", codes: Buffer, scales: Buffer, dtype: str):
+        _holds("codes", codes, codes.len, "i8")
+        _holds("scales", scales, -(-codes.len // self.BLOCK), "f32")
+        self.device = device
+        self.codes = codes
+        self.scales = scales
+        self.dtype = dtype  # of the buffer it was made from
+
+    @property
+    def len(self) -> int:
+        return self.codes.len
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.scales.nbytes
+
+
 class Graph:
     """An instantiated, replayable capture (`LazyCudaGraph`, src/devices/cuda/lazy.rs:10-29)."""
 
@@ -317,6 +363,57 @@ class HIP:
         src = _wrap(lhs_grad_fn(Resolve("x"))).to_cl_source(lhs.dtype)
         kernel = self.compile(capi.KIND_UNARY_GRAD, lhs.dtype, src, ("x",))
         self._check(self.lib.custos_hip_add_unary_grad(self.handle, kernel, lhs.ptr, lhs_grad.ptr, out_grad.ptr, lhs.len))
+
+    # -- operators of a training step --
+    def group_norm(self, x: Buffer, gamma: Buffer | None, beta: Buffer | None, shape, groups: int, activation: str = "none",
+                   eps: float = 1e-5, out: Buffer | None = None, stats: Buffer | None = None, x_pitch: int | None = None,
+                   out_pitch: int | None = None):
+        """Group norm with an activation over channels-last data (`custos_hip_group_norm`): `shape` is
+        (samples, positions, channels), the pitches are elements from one position to the next.  Returns
+        (out, stats); `stats` (f32, mean and 1/deviation of every sample and group) goes to the gradient."""
+        samples, positions, channels = shape
+        x_pitch = channels if x_pitch is None else x_pitch
+        out_pitch = channels if out_pitch is None else out_pitch
+        if out is None:
+            out = self.alloc(_rows_len(samples * positions, channels, out_pitch), x.dtype, zeroed=False)
+        if stats is None:
+            stats = self.alloc(samples * groups * 2, "f32", zeroed=False)
+        desc = _group_norm_desc(x.dtype, gamma, beta, shape, groups, activation, eps, 0)
+        _holds("x", x, _rows_len(samples * positions, channels, x_pitch), x.dtype)
+        _holds("out", out, _rows_len(samples * positions, channels, out_pitch), x.dtype)
+        _holds("stats", stats, samples * groups * 2, "f32")
+        self._check(self.lib.custos_hip_group_norm(self.handle, desc, x.ptr, x_pitch, gamma.ptr if gamma is not None else 0,
+                                                   beta.ptr if beta is not None else 0, out.ptr, out_pitch, stats.ptr))
+        return out, stats
+
+    def add_group_norm_grad(self, x, stats: Buffer, gamma: Buffer | None, beta: Buffer | None, out_grad: Buffer,
+                            x_grad: Buffer | None, gamma_grad: Buffer | None, beta_grad: Buffer | None, shape, groups: int,
+                            activation: str = "none", overwrite: bool = False, x_pitch: int | None = None,
+                            out_grad_pitch: int | None = None, x_grad_pitch: int | None = None) -> None:
+        """The gradients of `group_norm`, added to what the operands hold like `add_unary_grad`'s, or with
+        `overwrite` stored.  `x` is the forward pass's input or an 8-bit checkpoint of it; gradients that are
+        None are not computed."""
+        samples, positions, channels = shape
+        rows = samples * positions
+        saved = isinstance(x, Checkpoint8)
+        x_pitch = channels if x_pitch is None else x_pitch
+        out_grad_pitch = channels if out_grad_pitch is None else out_grad_pitch
+        x_grad_pitch = channels if x_grad_pitch is None else x_grad_pitch
+        desc = _group_norm_desc(x.dtype, gamma, beta, shape, groups, activation, 1.0, capi.GRAD_OVERWRITE if overwrite else 0)
+        if saved:
+            if x.len != rows * channels or x_pitch != channels:
+                raise ValueError(f"the checkpoint holds {x.len} values, the shape needs {rows * channels} without a pitch")
+        else:
+            _holds("x", x, _rows_len(rows, channels, x_pitch), x.dtype)
+        _holds("stats", stats, samples * groups * 2, "f32")
+        _holds("out_grad", out_grad, _rows_len(rows, channels, out_grad_pitch), x.dtype)
+        _holds("x_grad", x_grad, _rows_len(rows, channels, x_grad_pitch), x.dtype)
+        _holds("gamma_grad", gamma_grad, channels, "f32")
+        _holds("beta_grad", beta_grad, channels, "f32")
+        self._check(self.lib.custos_hip_add_group_norm_grad(
+            self.handle, desc, 0 if saved else x.ptr, x_pitch, x.codes.ptr if saved else 0, x.scales.ptr if saved else 0, stats.ptr,
+            gamma.ptr if gamma is not None else 0, beta.ptr if beta is not None else 0, out_grad.ptr, out_grad_pitch, x_grad.ptr if x_grad is not None else 0, x_grad_pitch,
+            gamma_grad.ptr if gamma_grad is not None else 0, beta_grad.ptr if beta_grad is not None else 0))
 
     # -- caller-written kernels (`launch_kernel` / `launch_kernel1d`, src/devices/cuda/cuda_device.rs:85-112) --
     def _source_args(self, args):

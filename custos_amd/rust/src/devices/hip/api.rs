@@ -31,6 +31,18 @@ pub const GRAPH_EDGES_PER_NODE: i32 = 1;
 pub const GRAPH_EDGES_CHAIN: i32 = 2;
 pub const GRAPH_EDGES_CHAIN_BY_LEVEL: i32 = 3;
 
+/// `custos_hip_group_norm_desc`
+#[repr(C)]
+pub struct HipGroupNormDesc {
+    pub dtype: i32, pub param_dtype: i32, pub activation: i32, pub flags: i32, pub samples: u64, pub positions: u64,
+    pub channels: u64, pub groups: u64, pub eps: f64,
+}
+pub const ACT_NONE: i32 = 0;
+pub const ACT_RELU: i32 = 1;
+pub const ACT_SILU: i32 = 2;
+pub const ACT_GELU: i32 = 3;
+pub const GRAD_OVERWRITE: i32 = 1;
+
 #[link(name = "custos_hip")]
 extern "C" {
     pub fn custos_hip_device_count(count: *mut i32) -> i32;
@@ -117,6 +129,12 @@ extern "C" {
     pub fn custos_hip_compile_stats(dev: *mut HipDeviceHandle, units: *mut u64, milliseconds: *mut f64) -> i32;
     pub fn custos_hip_add_unary_grad(dev: *mut HipDeviceHandle, kernel: *mut HipKernel, lhs: u64, lhs_grad: u64,
                                      out_grad: u64, n: usize) -> i32;
+    pub fn custos_hip_group_norm(dev: *mut HipDeviceHandle, desc: *const HipGroupNormDesc, x: u64, x_pitch: u64, gamma: u64,
+                                 beta: u64, out: u64, out_pitch: u64, stats: u64) -> i32;
+    pub fn custos_hip_add_group_norm_grad(dev: *mut HipDeviceHandle, desc: *const HipGroupNormDesc, x: u64, x_pitch: u64,
+                                          codes: u64, scales: u64, stats: u64, gamma: u64, beta: u64, out_grad: u64,
+                                          out_grad_pitch: u64, x_grad: u64, x_grad_pitch: u64, gamma_grad: u64,
+                                          beta_grad: u64) -> i32;
     pub fn custos_hip_capture_begin(dev: *mut HipDeviceHandle) -> i32;
     pub fn custos_hip_capture_end(dev: *mut HipDeviceHandle, graph: *mut *mut HipGraph) -> i32;
     pub fn custos_hip_capture_end_reuse(dev: *mut HipDeviceHandle, previous: *mut HipGraph,

@@ -418,6 +418,57 @@ int32_t custos_hip_check_operand_sets(const uint64_t *operands, int32_t operands
  * a graph build the ones its nodes use, this call the second.  No counterpart in the reference. */
 int32_t custos_hip_kernel_prepare_merged(custos_hip_device *dev, custos_hip_kernel *kernel);
 
+/* ---- operators of a training step ----
+ *
+ * No counterparts in the reference.  They follow the rules of the launches above: everything runs on
+ * the device handle's compute stream in call order, may be recorded and replayed, and is checked
+ * before anything is launched.  What an operator needs besides its operands it takes from a work
+ * area the device keeps.  An operand that is written must not overlap another one; where a call
+ * says so it may be exactly one of the operands read, and rows with a pitch may lie side by side in
+ * one wider tensor.  Sums are held in f32 or f64 in a fixed order: the same call gives the same bits. */
+
+enum custos_hip_activation {
+    CUSTOS_HIP_ACT_NONE = 0,
+    CUSTOS_HIP_ACT_RELU = 1,
+    CUSTOS_HIP_ACT_SILU = 2, /* z / (1 + exp(-z)) */
+    CUSTOS_HIP_ACT_GELU = 3  /* z / 2 * (1 + erf(z / sqrt 2)) */
+};
+
+/* Gradients are added to what the operand holds, like custos_hip_add_unary_grad's, unless this is
+ * set: then they are stored, so that a first gradient needs no cleared operand and no read of it. */
+#define CUSTOS_HIP_GRAD_OVERWRITE 1
+
+/* x is [samples][positions][channels], `groups` groups of channels / groups neighbouring channels. */
+typedef struct custos_hip_group_norm_desc {
+    int32_t dtype;       /* of x, out and their gradients: CUSTOS_HIP_F32, _F16 or _BF16 */
+    int32_t param_dtype; /* of gamma and beta: CUSTOS_HIP_F32, or the same as dtype */
+    int32_t activation;
+    int32_t flags;       /* the gradient's: 0 or CUSTOS_HIP_GRAD_OVERWRITE */
+    uint64_t samples, positions, channels, groups;
+    double eps;
+} custos_hip_group_norm_desc;
+
+/* Group norm with an activation, channels last.  With M = positions * channels / groups values per
+ * sample and group: h = (x - mean) / sqrt(var + eps) (var over M, not M - 1), out = act(h * gamma +
+ * beta), rounded once.  Pitches: elements from one position to the next (>= channels).  gamma or
+ * beta 0: ones, zeros.  `stats` receives mean and 1 / sqrt(var + eps) as f32
+ * [samples][groups][2], which the gradient takes.  out may be x exactly.  No samples or no positions:
+ * nothing is done.  NaN and infinities in a group make that group's results NaN, as the formula does. */
+int32_t custos_hip_group_norm(custos_hip_device *dev, const custos_hip_group_norm_desc *desc, uint64_t x,
+                              uint64_t x_pitch, uint64_t gamma, uint64_t beta, uint64_t out,
+                              uint64_t out_pitch, uint64_t stats);
+/* Its gradients.  x is given as values (`x`, `x_pitch`; codes and scales 0) or as an 8-bit checkpoint
+ * of the whole of it ([samples * positions * channels] codes, their scales; x 0; the pitch of such an x is
+ * `channels`, `x_pitch` is not looked at).  x_grad has the element type of x; gamma_grad and
+ * beta_grad are f32 [channels].  Each of the three may be 0: not wanted.  With
+ * CUSTOS_HIP_GRAD_OVERWRITE x_grad may be x or out_grad exactly.  No samples or no positions: the
+ * gradients of gamma and beta are zeros (stored or added), nothing else is done. */
+int32_t custos_hip_add_group_norm_grad(custos_hip_device *dev, const custos_hip_group_norm_desc *desc, uint64_t x,
+                                       uint64_t x_pitch, uint64_t codes, uint64_t scales, uint64_t stats,
+                                       uint64_t gamma, uint64_t beta, uint64_t out_grad,
+                                       uint64_t out_grad_pitch, uint64_t x_grad, uint64_t x_grad_pitch,
+                                       uint64_t gamma_grad, uint64_t beta_grad);
+
 /* ---- lazy run: capture once, replay (src/devices/cuda/lazy.rs:10-72) ---- */
 
 /* LazySetup::lazy_setup: from here on launches/clears/copies are recorded, not run.

@@ -1,0 +1,140 @@
+"""What the training operators refuse, checked on the host before a device is needed: a call without a device
+handle that passes every check fails for the missing handle, one that does not names what is wrong."""
+import numpy as np
+import pytest
+
+from custos_amd import capi
+
+F32, F16, BF16, I32 = (capi.DTYPES[k][0] for k in ("f32", "f16", "bf16", "i32"))
+BASE = 1 << 32  # addresses that are never touched
+
+
+def refused(rc, code, text):
+    assert rc == code, (rc, capi.last_error(None))
+    assert text in capi.last_error(None), capi.last_error(None)
+
+
+def gn_desc(**over):
+    d = dict(dtype=F32, param_dtype=F32, activation=0, flags=0, samples=2, positions=10, channels=8, groups=2, eps=1e-5)
+    return capi.GroupNormDesc(**{**d, **over})
+
+
+def gn(desc=None, x=BASE, x_pitch=8, gamma=BASE + 0x10000, beta=BASE + 0x20000, out=BASE + 0x30000, out_pitch=8, stats=BASE + 0x40000):
+    lib = capi.load_library()
+    return lib.custos_hip_group_norm(None, desc, x, x_pitch, gamma, beta, out, out_pitch, stats)
+
+
+def gn_grad(desc=None, x=BASE, x_pitch=8, codes=0, scales=0, stats=BASE + 0x10000, gamma=0, beta=0, out_grad=BASE + 0x20000, og_pitch=8,
+            x_grad=BASE + 0x30000, xg_pitch=8, gamma_grad=BASE + 0x40000, beta_grad=BASE + 0x50000):
+    lib = capi.load_library()
+    return lib.custos_hip_add_group_norm_grad(None, desc, x, x_pitch, codes, scales, stats, gamma, beta, out_grad, og_pitch, x_grad,
+                                              xg_pitch, gamma_grad, beta_grad)
+
+
+INVALID, OVERLAP, LARGE = capi.ERR_INVALID_ARGUMENT, capi.ERR_BAD_OVERLAP, capi.ERR_TOO_LARGE
+
+
+def test_calls_that_pass_every_check_need_a_device():
+    refused(gn(gn_desc()), INVALID, "device handle is null")
+    refused(gn(gn_desc(), gamma=0, beta=0), INVALID, "device handle is null")
+    refused(gn(gn_desc(samples=0)), INVALID, "device handle is null")
+    refused(gn(gn_desc(), out=BASE), INVALID, "device handle is null")  # in place
+    refused(gn(gn_desc(), x_pitch=16, out_pitch=16, out=BASE + 32), INVALID, "device handle is null")  # side by side
+    refused(gn_grad(gn_desc()), INVALID, "device handle is null")
+    refused(gn_grad(gn_desc(flags=1), x_grad=BASE), INVALID, "device handle is null")
+    refused(gn_grad(gn_desc(), x=0, codes=BASE, scales=BASE + 0x8000), INVALID, "device handle is null")
+    refused(gn_grad(gn_desc(), x_grad=0, gamma_grad=0, beta_grad=0), INVALID, "device handle is null")
+
+
+@pytest.mark.parametrize("over, text", [
+    (dict(dtype=I32), "f32, f16 or bf16"),
+    (dict(dtype=F16, param_dtype=BF16), "f32 or of the element type"),
+    (dict(activation=9), "unknown activation"),
+    (dict(activation=-1), "unknown activation"),
+    (dict(flags=2), "unknown flag"),
+    (dict(channels=0), "divide into the groups"),
+    (dict(groups=0), "divide into the groups"),
+    (dict(groups=3), "divide into the groups"),
+    (dict(eps=0.0), "eps is positive"),
+    (dict(eps=-1.0), "eps is positive"),
+    (dict(eps=float("nan")), "eps is positive"),
+    (dict(eps=float("inf")), "eps is positive"),
+])
+def test_group_norm_descriptions(over, text):
+    refused(gn(gn_desc(**over)), INVALID, text)
+    refused(gn_grad(gn_desc(**over)), INVALID, text)
+
+
+def test_group_norm_sizes_beyond_any_memory():
+    for over in (dict(channels=1 << 40, groups=1), dict(samples=1 << 40), dict(positions=1 << 60), dict(samples=1 << 30, positions=1 << 39)):
+        refused(gn(gn_desc(**over)), LARGE, "beyond any memory")
+        refused(gn_grad(gn_desc(**over)), LARGE, "beyond any memory")
+
+
+@pytest.mark.parametrize("over, code, text", [
+    (dict(x=0), INVALID, "x is a null address"),
+    (dict(out=0), INVALID, "out is a null address"),
+    (dict(stats=0), INVALID, "stats is a null address"),
+    (dict(x=BASE + 2), INVALID, "x is not aligned"),
+    (dict(gamma=BASE + 0x10001), INVALID, "gamma is not aligned"),
+    (dict(x_pitch=7), INVALID, "pitch shorter"),
+    (dict(out_pitch=0), INVALID, "pitch shorter"),
+    (dict(x=2**64 - 64), INVALID, "wraps around"),
+    (dict(x_pitch=1 << 60), LARGE, "larger than any memory"),
+    (dict(out=BASE + 32), OVERLAP, "out overlaps x"),
+    (dict(out=BASE, out_pitch=16), OVERLAP, "out overlaps x"),
+    (dict(out=BASE + 0x10000), OVERLAP, "out overlaps gamma"),
+    (dict(stats=BASE + 0x30000), OVERLAP, "out overlaps stats"),
+    (dict(stats=BASE), OVERLAP, "stats overlaps x"),
+    (dict(x_pitch=12, out_pitch=12, out=BASE + 32), OVERLAP, "out overlaps x"),  # slices of 8 in rows of 12
+])
+def test_group_norm_operands(over, code, text):
+    refused(gn(gn_desc(), **over), code, text)
+
+
+@pytest.mark.parametrize("over, code, text", [
+    (dict(codes=BASE, scales=BASE), INVALID, "either as values or as codes"),
+    (dict(x=0), INVALID, "either as values or as codes"),
+    (dict(x=0, codes=BASE), INVALID, "either as values or as codes"),
+    (dict(stats=0), INVALID, "stats is a null address"),
+    (dict(out_grad=0), INVALID, "out_grad is a null address"),
+    (dict(gamma_grad=BASE + 0x40002), INVALID, "gamma_grad is not aligned"),
+    (dict(x_grad=BASE), OVERLAP, "x_grad overlaps x"),  # it is added to: not in place
+    (dict(beta_grad=BASE + 0x40000), OVERLAP, "gamma_grad overlaps beta_grad"),
+    (dict(og_pitch=1), INVALID, "pitch shorter"),
+])
+def test_group_norm_gradient_operands(over, code, text):
+    refused(gn_grad(gn_desc(), **over), code, text)
+
+
+def test_forward_takes_no_flags():
+    refused(gn(gn_desc(flags=1)), INVALID, "no flags")
+    refused(gn(None), INVALID, "description is null")
+
+
+def test_group_norm_formula_against_differences():
+    """The gradient formula the kernels are tested with, against differences of the forward formula."""
+    import operator_refs as refs
+    rng = np.random.default_rng(0)
+    n, p, c, groups = 2, 3, 6, 2
+    x, og = rng.normal(size=(n, p, c)), rng.normal(size=(n, p, c))
+    gamma, beta = rng.normal(size=c), rng.normal(size=c)
+    for activation in ("none", "relu", "silu", "gelu"):
+        _, mean, rstd, z = refs.group_norm(x, gamma, beta, groups, activation, 1e-3)
+        assert np.abs(z).min() > 1e-4  # (no difference steps over relu's corner)
+        (xg, gg, bg), _ = refs.group_norm_grad(x, mean, rstd, gamma, beta, og, groups, activation)
+
+        def loss(x_, g_, b_):
+            return float((refs.group_norm(x_, g_, b_, groups, activation, 1e-3)[0] * og).sum())
+
+        step = 1e-5
+        for which, grad in ((0, xg), (1, gg), (2, bg)):
+            args = [x, gamma, beta]
+            for at in np.ndindex(args[which].shape):
+                moved = []
+                for sign in (1, -1):
+                    a = [v.copy() for v in args]
+                    a[which][at] += sign * step
+                    moved.append(loss(*a))
+                # (error of a central difference: step^2 times a third derivative, and roundings over the step)
+                assert abs((moved[0] - moved[1]) / (2 * step) - grad[at]) < 1e-6, (activation, which, at)
