@@ -7,6 +7,7 @@ import os
 
 KIND_APPLY = 0
 KIND_UNARY_GRAD = 1
+KIND_SAVE8, KIND_RESTORE8, KIND_UNARY_GRAD8 = 4, 5, 6
 
 ALLOC_ZEROED = 0
 ALLOC_UNINIT = 1
@@ -187,6 +188,9 @@ PROTOTYPES = {
     "custos_hip_set_graph_verify": (C.c_int32, [_P, C.c_int32]),
     "custos_hip_graph_edge_count": (C.c_int32, [_P, C.POINTER(C.c_size_t)]),
     "custos_hip_graph_destroy": (C.c_int32, [_P, _P]),
+    "custos_hip_checkpoint8_save": (C.c_int32, [_P, _P] + [C.c_uint64] * 4 + [C.c_size_t]),
+    "custos_hip_checkpoint8_restore": (C.c_int32, [_P, _P] + [C.c_uint64] * 3 + [C.c_size_t]),
+    "custos_hip_add_unary_grad8": (C.c_int32, [_P, _P] + [C.c_uint64] * 4 + [C.c_size_t, C.c_int32]),
     "custos_hip_group_norm": (C.c_int32, [_P, C.POINTER(GroupNormDesc)] + [C.c_uint64] * 7),
     "custos_hip_add_group_norm_grad": (C.c_int32, [_P, C.POINTER(GroupNormDesc)] + [C.c_uint64] * 13),
     "custos_hip_timer_begin": (C.c_int32, [_P]),

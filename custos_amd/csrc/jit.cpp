@@ -99,7 +99,7 @@ int32_t spec_from_c(custos_hip_device* dev, int32_t kind, int32_t dtype, const c
                     const char* const* markers, int32_t n_markers, const Tuning& tuning,
                     bool literals_in_code, KernelSpec* spec, bool with_source = true) {
     if (!src) return set_error(dev, CUSTOS_HIP_ERR_INVALID_ARGUMENT, "expression source is null");
-    if (kind != CUSTOS_HIP_KIND_APPLY && kind != CUSTOS_HIP_KIND_UNARY_GRAD)
+    if (kind != CUSTOS_HIP_KIND_APPLY && kind != CUSTOS_HIP_KIND_UNARY_GRAD && !checkpoint8_kind(static_cast<Kind>(kind)))
         return set_error(dev, CUSTOS_HIP_ERR_INVALID_ARGUMENT, "unknown kernel kind");
     if (!dtype_valid(dtype)) return set_error(dev, CUSTOS_HIP_ERR_INVALID_ARGUMENT, "unknown element type");
     std::vector<std::string> m;
@@ -112,10 +112,12 @@ int32_t spec_from_c(custos_hip_device* dev, int32_t kind, int32_t dtype, const c
     return CUSTOS_HIP_OK;
 }
 
-// The three translation units of a generated kernel, one after the other (generated on the way).
+int units_of(const KernelSpec& spec) { return checkpoint8_kind(spec.kind) ? 1 : kEntrySets; }
+
+// The translation units of a generated kernel, one after the other (generated on the way).
 std::string all_units(KernelSpec* spec) {
     std::string text;
-    for (int w = 0; w < kEntrySets; w++) {
+    for (int w = 0; w < units_of(*spec); w++) {
         ParseError err;
         if (spec->source[w].empty()) (void)emit_kernel_source(spec, &err, static_cast<EntrySet>(w));
         // (every unit starts with a line that spells the expression: once is enough here)
@@ -543,7 +545,7 @@ int32_t custos_hip_expr_build_code_object(int32_t kind, int32_t dtype, const cha
     if (rc != CUSTOS_HIP_OK) return rc;
     (void)all_units(&spec);
     size_t total = 0;
-    for (int w = 0; w < kEntrySets; w++) {
+    for (int w = 0; w < units_of(spec); w++) {
         std::vector<char> code;
         rc = compile_to_code_object(nullptr, spec, "gfx950", &code, static_cast<EntrySet>(w));
         if (rc != CUSTOS_HIP_OK) return rc;

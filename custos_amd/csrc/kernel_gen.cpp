@@ -631,6 +631,138 @@ struct KernelText {
     }
 };
 
+// ---- 8-bit checkpoints ----
+//
+// 128 neighbouring elements share a scale: with top the largest finite magnitude among them, the code of x is
+// x * (127 / top) rounded to the nearest whole number (ties to even) and stands for code * (top * (1 / 127)), all
+// in f32.  Code -128 stands for NaN and is given to what is not finite, so that an overflowed activation shows in
+// the gradient instead of passing for a large one; a block whose top is below 2^-100 is kept as zeros (127 / top
+// would leave f32's range soon below it).
+//
+// A lane holds a 16-byte vector, 16 lanes (f32: 32) a block: the largest magnitude crosses lanes in registers.
+// One pass, bound by memory: the input is read once for the result and for the checkpoint.  Addresses are
+// multiples of the element size and no more (a buffer may be a slice), which gfx950's loads and stores take.
+std::string checkpoint8_source(const KernelSpec& k, const std::string& body) {
+    std::string s;
+    s += "// generated by custos-hip: " + to_cl_source(k.expr, k.markers, &k.consts) + "\n";
+    s += "#define CUSTOS_BT " + std::to_string(kCheckpoint8Threads) + "u\n";
+    s += "#define CUSTOS_UNROLL " + std::to_string(kCheckpoint8Unroll) + "\n";
+    s += "#define CUSTOS_VEC " + std::to_string(k.vec_elems) + "\n";
+    s += prelude(k.dtype, k.vec_elems, k.consts.n_params);
+    s += expr_fn(k, body);
+    if (k.kind == Kind::UnaryGrad8) s += grad_fn(k.dtype);
+    s += R"(typedef vec_t vec_any __attribute__((aligned(sizeof(S))));
+typedef signed char codes_t __attribute__((ext_vector_type(CUSTOS_VEC)));
+typedef codes_t codes_any __attribute__((aligned(1)));
+// A vector that may end behind the data: `left` elements of it exist.
+static __device__ __forceinline__ vec_t custos_get(const S* p, const u64 i, const u64 n) {
+    if (i + CUSTOS_VEC <= n) return *(const vec_any*)(p + i);
+    vec_t v = (vec_t)(S)0;
+    for (int k = 0; k < CUSTOS_VEC; k++)
+        if (i + k < n) v[k] = p[i + k];
+    return v;
+}
+static __device__ __forceinline__ void custos_put(S* p, const u64 i, const u64 n, const vec_t v) {
+    if (i + CUSTOS_VEC <= n) {
+        *(vec_any*)(p + i) = v;
+        return;
+    }
+    for (int k = 0; k < CUSTOS_VEC; k++)
+        if (i + k < n) p[i + k] = v[k];
+}
+)";
+    if (k.kind == Kind::Save8) {
+        s += R"(// The largest value of the lanes that share a block (16, or 32 with 4 elements a lane).
+static __device__ __forceinline__ float custos_block_max(float v) {
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, true)));   // lane ^ 1
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, true)));   // lane ^ 2
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true)));  // 7 - lane of 8
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true)));  // 15 - lane of 16
+    if (CUSTOS_VEC == 4) v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401f)));  // lane ^ 16
+    return v;
+}
+)";
+        s += "extern \"C\" __global__ void __launch_bounds__(CUSTOS_BT)\n" + k.name +
+             "(const S* x, S* out, signed char* codes, float* scales, const u64 n, CUSTOS_KC_ENTRY const u64 mode) {\n";
+        s += R"(    const u64 first = ((u64)blockIdx.x * CUSTOS_UNROLL * CUSTOS_BT + threadIdx.x) * CUSTOS_VEC;
+    vec_t v[CUSTOS_UNROLL];
+#pragma unroll
+    for (int u = 0; u < CUSTOS_UNROLL; u++) v[u] = custos_get(x, first + (u64)u * CUSTOS_BT * CUSTOS_VEC, n);
+#pragma unroll
+    for (int u = 0; u < CUSTOS_UNROLL; u++) {
+        const u64 i = first + (u64)u * CUSTOS_BT * CUSTOS_VEC;
+        float a[CUSTOS_VEC];
+        float top = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int k = 0; k < CUSTOS_VEC; k++) {
+            a[k] = custos_load(v[u][k]);
+            finite = finite && fabsf(a[k]) < __builtin_inff();
+            top = fmaxf(top, fabsf(a[k]));
+        }
+        if (!finite) {
+            top = 0.0f;
+            for (int k = 0; k < CUSTOS_VEC; k++) top = fmaxf(top, fabsf(a[k]) < __builtin_inff() ? fabsf(a[k]) : 0.0f);
+        }
+        top = custos_block_max(top);
+        const bool kept = top >= 0x1p-100f;
+        const float step = kept ? 127.0f / top : 0.0f;
+        codes_t c;
+#pragma unroll
+        for (int k = 0; k < CUSTOS_VEC; k++) c[k] = (signed char)(int)__builtin_rintf(a[k] * step);
+        if (!finite)
+            for (int k = 0; k < CUSTOS_VEC; k++)
+                if (!(fabsf(a[k]) < __builtin_inff())) c[k] = -128;
+        if (i + CUSTOS_VEC <= n) *(codes_any*)(codes + i) = c;
+        else
+            for (int k = 0; k < CUSTOS_VEC; k++)
+                if (i + k < n) codes[i + k] = c[k];
+        if ((i & 127) == 0 && i < n) scales[i >> 7] = kept ? top * 0x1.020408p-7f : 0.0f;
+        if (mode & 1) {
+            vec_t r;
+#pragma unroll
+            for (int k = 0; k < CUSTOS_VEC; k++) r[k] = custos_store(custos_expr(a[k] CUSTOS_KC_ARG));
+            custos_put(out, i, n, r);
+        }
+    }
+}
+)";
+        return s;
+    }
+    s += "static __device__ __forceinline__ C custos_restore(const signed char code, const float scale) {\n"
+         "    const float v = code == -128 ? __builtin_nanf(\"\") : (float)code * scale;\n";
+    s += dtype_rounds_per_node(k.dtype) ? "    return custos_round(v);\n}\n" : "    return v;\n}\n";
+    s += R"(static __device__ __forceinline__ codes_t custos_codes(const signed char* p, const u64 i, const u64 n) {
+    if (i + CUSTOS_VEC <= n) return *(const codes_any*)(p + i);
+    codes_t c = (codes_t)(signed char)0;
+    for (int k = 0; k < CUSTOS_VEC; k++)
+        if (i + k < n) c[k] = p[i + k];
+    return c;
+}
+)";
+    const bool grad = k.kind == Kind::UnaryGrad8;
+    s += "extern \"C\" __global__ void __launch_bounds__(CUSTOS_BT)\n" + k.name + "(const signed char* codes, const float* scales, S* out, " +
+         (grad ? "const S* out_grad, " : "") + "const u64 n, CUSTOS_KC_ENTRY const u64 mode) {\n";
+    s += "    const u64 first = ((u64)blockIdx.x * CUSTOS_UNROLL * CUSTOS_BT + threadIdx.x) * CUSTOS_VEC;\n"
+         "    codes_t c[CUSTOS_UNROLL];\n    float scale[CUSTOS_UNROLL];\n";
+    if (grad) s += "    vec_t o[CUSTOS_UNROLL], g[CUSTOS_UNROLL];\n";
+    s += "#pragma unroll\n    for (int u = 0; u < CUSTOS_UNROLL; u++) {\n"
+         "        const u64 i = first + (u64)u * CUSTOS_BT * CUSTOS_VEC;\n"
+         "        c[u] = custos_codes(codes, i, n);\n"
+         "        scale[u] = i < n ? scales[i >> 7] : 0.0f;\n";
+    if (grad) s += "        o[u] = custos_get(out_grad, i, n);\n        if (mode & 1) g[u] = custos_get(out, i, n);\n";
+    s += "    }\n#pragma unroll\n    for (int u = 0; u < CUSTOS_UNROLL; u++) {\n        vec_t r;\n";
+    const std::string f = "custos_expr(custos_restore(c[u][k], scale[u]) CUSTOS_KC_ARG)";
+    const std::string each = "#pragma unroll\n        for (int k = 0; k < CUSTOS_VEC; k++) r[k] = custos_store(";
+    if (!grad)
+        s += each + f + ");\n";
+    else
+        s += "        if (mode & 1) {\n" + each + "custos_grad(custos_load(g[u][k]), custos_load(o[u][k]), " + f + "));\n        } else {\n" +
+             each + "custos_load(o[u][k]) * " + f + ");\n        }\n";
+    s += "        custos_put(out, first + (u64)u * CUSTOS_BT * CUSTOS_VEC, n, r);\n    }\n    (void)mode;\n}\n";
+    return s;
+}
+
 }  // namespace
 
 bool build_kernel_spec(Kind kind, DType dtype, const std::string& src,
@@ -644,9 +776,15 @@ bool build_kernel_spec(Kind kind, DType dtype, const std::string& src,
     if (tuning.eq_as_leq)
         for (Node& n : k.expr.nodes)
             if (n.op == Op::Eq) n.op = Op::LEq;
-    if (kind == Kind::UnaryGrad && k.expr.n_vars != 1) {
+    if ((kind == Kind::UnaryGrad || checkpoint8_kind(kind)) && k.expr.n_vars != 1) {
         err->code = CUSTOS_HIP_ERR_ARITY_MISMATCH;
-        err->message = "a unary gradient expression takes exactly one marker";
+        err->message = kind == Kind::UnaryGrad ? "a unary gradient expression takes exactly one marker"
+                                               : "an expression over an 8-bit checkpoint takes exactly one marker";
+        return false;
+    }
+    if (checkpoint8_kind(kind) && (!dtype_is_float(dtype) || dtype == DType::F64)) {
+        err->code = CUSTOS_HIP_ERR_EXPR_UNSUPPORTED;
+        err->message = "8-bit checkpoints hold f32, f16 and bf16 values";
         return false;
     }
     // Vectors per thread left open: the kernel holds a tile function for two and for one, and
@@ -672,7 +810,8 @@ bool build_kernel_spec(Kind kind, DType dtype, const std::string& src,
                                                   "f16n", "bf16n"};
         char hex[17];
         std::snprintf(hex, sizeof hex, "%016llx", static_cast<unsigned long long>(k.hash));
-        k.name = std::string(kind == Kind::Apply ? "custos_apply_" : "custos_unary_grad_") +
+        k.name = std::string(kind == Kind::Apply ? "custos_apply_" : kind == Kind::Save8 ? "custos_save8_" : kind == Kind::Restore8 ? "custos_restore8_"
+                                                              : kind == Kind::UnaryGrad8 ? "custos_unary_grad8_" : "custos_unary_grad_") +
                  dtype_names[static_cast<int>(dtype)] + "_" + hex;
     }
 
@@ -684,6 +823,16 @@ bool build_kernel_spec(Kind kind, DType dtype, const std::string& src,
 bool emit_kernel_source(KernelSpec* spec, ParseError* err, EntrySet which) {
     KernelSpec& k = *spec;
     std::string body;
+    if (checkpoint8_kind(k.kind)) {
+        if (which != EntrySet::Single) {
+            err->code = CUSTOS_HIP_ERR_KIND_MISMATCH;
+            err->message = "a kernel over 8-bit checkpoints has no entry point for merged launches";
+            return false;
+        }
+        if (!emit_expr_body(k.expr, k.dtype, k.consts, &body, err)) return false;
+        k.source[0] = checkpoint8_source(k, body);
+        return true;
+    }
     if (k.kind == Kind::Chain) {
         // (the stage functions are emitted by KernelText; here only what cannot be compiled is found)
         for (const ChainStage& stage : k.stages) {

@@ -20,7 +20,16 @@ enum class Kind : int32_t {
     UnaryGrad = 1,
     Source = 2,  // caller-written kernel source
     Chain = 3,   // several apply expressions in one kernel, every one with its own output (made when a graph is built)
+    Save8 = 4,       // apply that also writes an 8-bit checkpoint of its input
+    Restore8 = 5,    // apply to the values an 8-bit checkpoint stands for
+    UnaryGrad8 = 6,  // unary gradient whose input is an 8-bit checkpoint
 };
+
+// The kinds that work on 8-bit checkpoints (custos_hip_checkpoint8_*): one marker, one entry point.
+inline bool checkpoint8_kind(Kind kind) { return kind == Kind::Save8 || kind == Kind::Restore8 || kind == Kind::UnaryGrad8; }
+constexpr int kCheckpoint8Block = 128;    // elements that share a scale
+constexpr int kCheckpoint8Threads = 256;  // per workgroup
+constexpr int kCheckpoint8Unroll = 2;     // 16-byte vectors per thread
 
 struct Tuning {
     // Launch shape of the generated kernels.  Workgroups of 64 or 128 threads

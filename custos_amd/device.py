@@ -364,6 +364,55 @@ class HIP:
         kernel = self.compile(capi.KIND_UNARY_GRAD, lhs.dtype, src, ("x",))
         self._check(self.lib.custos_hip_add_unary_grad(self.handle, kernel, lhs.ptr, lhs_grad.ptr, out_grad.ptr, lhs.len))
 
+    # -- 8-bit checkpoints --
+    def alloc_checkpoint8(self, length: int, dtype: str = "f32") -> Checkpoint8:
+        """Room for the checkpoint of a buffer of `length` elements."""
+        return Checkpoint8(self, self.alloc(length, "i8", zeroed=False), self.alloc(-(-length // Checkpoint8.BLOCK), "f32", zeroed=False), dtype)
+
+    def _room8(self, x: Buffer, into: Checkpoint8 | None) -> Checkpoint8:
+        if into is None:
+            return self.alloc_checkpoint8(x.len, x.dtype)
+        if into.len != x.len or into.dtype != x.dtype:
+            raise ValueError(f"the checkpoint is for {into.len} x {into.dtype}, the buffer is {x.len} x {x.dtype}")
+        return into
+
+    def checkpoint8(self, x: Buffer, into: Checkpoint8 | None = None) -> Checkpoint8:
+        """`x` kept in 8 bits (see `custos_hip_checkpoint8_save`)."""
+        into = self._room8(x, into)
+        kernel = self.compile(capi.KIND_SAVE8, x.dtype, "x", ("x",))
+        self._check(self.lib.custos_hip_checkpoint8_save(self.handle, kernel, x.ptr, 0, into.codes.ptr, into.scales.ptr, x.len))
+        return into
+
+    def apply_fn_checkpoint8(self, x: Buffer, f, out: Buffer | None = None, into: Checkpoint8 | None = None):
+        """`apply_fn` that also keeps its input in 8 bits, in one pass; returns (out, checkpoint)."""
+        _same_shape(x, out)
+        into = self._room8(x, into)
+        src = _wrap(f(Resolve("x"))).to_cl_source(x.dtype)
+        kernel = self.compile(capi.KIND_SAVE8, x.dtype, src, ("x",))
+        if out is None:
+            out = self.alloc(x.len, x.dtype, zeroed=False)
+        self._check(self.lib.custos_hip_checkpoint8_save(self.handle, kernel, x.ptr, out.ptr, into.codes.ptr, into.scales.ptr, x.len))
+        return out, into
+
+    def restore8(self, saved: Checkpoint8, f=None, out: Buffer | None = None) -> Buffer:
+        """The values a checkpoint stands for, or `f` of them, rounded to its element type."""
+        src = "x" if f is None else _wrap(f(Resolve("x"))).to_cl_source(saved.dtype)
+        kernel = self.compile(capi.KIND_RESTORE8, saved.dtype, src, ("x",))
+        if out is None:
+            out = self.alloc(saved.len, saved.dtype, zeroed=False)
+        _same_shape(saved, out)
+        self._check(self.lib.custos_hip_checkpoint8_restore(self.handle, kernel, saved.codes.ptr, saved.scales.ptr, out.ptr, saved.len))
+        return out
+
+    def add_unary_grad8(self, saved: Checkpoint8, lhs_grad: Buffer, out_grad: Buffer, lhs_grad_fn, overwrite: bool = False) -> None:
+        """`add_unary_grad` with the operation's input taken from its checkpoint; `overwrite` stores the
+        product instead of adding it."""
+        _same_shape(saved, lhs_grad, out_grad)
+        src = _wrap(lhs_grad_fn(Resolve("x"))).to_cl_source(saved.dtype)
+        kernel = self.compile(capi.KIND_UNARY_GRAD8, saved.dtype, src, ("x",))
+        self._check(self.lib.custos_hip_add_unary_grad8(self.handle, kernel, saved.codes.ptr, saved.scales.ptr, lhs_grad.ptr, out_grad.ptr,
+                                                        saved.len, capi.GRAD_OVERWRITE if overwrite else 0))
+
     # -- operators of a training step --
     def group_norm(self, x: Buffer, gamma: Buffer | None, beta: Buffer | None, shape, groups: int, activation: str = "none",
                    eps: float = 1e-5, out: Buffer | None = None, stats: Buffer | None = None, x_pitch: int | None = None,

@@ -21,6 +21,9 @@ pub struct HipTuning { pub block_threads: i32, pub unroll: i32, pub blocks_per_c
 
 pub const KIND_APPLY: i32 = 0;
 pub const KIND_UNARY_GRAD: i32 = 1;
+pub const KIND_SAVE8: i32 = 4;
+pub const KIND_RESTORE8: i32 = 5;
+pub const KIND_UNARY_GRAD8: i32 = 6;
 pub const ALLOC_ZEROED: i32 = 0;
 pub const ALLOC_UNINIT: i32 = 1;
 pub const LITERALS_ADAPTIVE: i32 = 0;
@@ -129,6 +132,12 @@ extern "C" {
     pub fn custos_hip_compile_stats(dev: *mut HipDeviceHandle, units: *mut u64, milliseconds: *mut f64) -> i32;
     pub fn custos_hip_add_unary_grad(dev: *mut HipDeviceHandle, kernel: *mut HipKernel, lhs: u64, lhs_grad: u64,
                                      out_grad: u64, n: usize) -> i32;
+    pub fn custos_hip_checkpoint8_save(dev: *mut HipDeviceHandle, kernel: *mut HipKernel, x: u64, out: u64, codes: u64, scales: u64,
+                                       n: usize) -> i32;
+    pub fn custos_hip_checkpoint8_restore(dev: *mut HipDeviceHandle, kernel: *mut HipKernel, codes: u64, scales: u64, out: u64,
+                                          n: usize) -> i32;
+    pub fn custos_hip_add_unary_grad8(dev: *mut HipDeviceHandle, kernel: *mut HipKernel, codes: u64, scales: u64, lhs_grad: u64,
+                                      out_grad: u64, n: usize, flags: i32) -> i32;
     pub fn custos_hip_group_norm(dev: *mut HipDeviceHandle, desc: *const HipGroupNormDesc, x: u64, x_pitch: u64, gamma: u64,
                                  beta: u64, out: u64, out_pitch: u64, stats: u64) -> i32;
     pub fn custos_hip_add_group_norm_grad(dev: *mut HipDeviceHandle, desc: *const HipGroupNormDesc, x: u64, x_pitch: u64,

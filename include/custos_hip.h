@@ -90,7 +90,13 @@ enum custos_hip_kind {
     CUSTOS_HIP_KIND_APPLY = 0,
     /* lhs_grad[i] += out_grad[i] * f(lhs[i]): `addUnaryGrad`
      * (src/devices/cuda/ops.rs:201-234). One marker. */
-    CUSTOS_HIP_KIND_UNARY_GRAD = 1
+    CUSTOS_HIP_KIND_UNARY_GRAD = 1,
+    /* 2 and 3 are used inside the library.  The kinds over 8-bit checkpoints (below), one marker each,
+     * f32, f16 and bf16 (and their per-node forms): out[i] = f(x[i]) that also saves x; out[i] = f(what
+     * is saved of x[i]); lhs_grad[i] += out_grad[i] * f(what is saved of lhs[i]). */
+    CUSTOS_HIP_KIND_SAVE8 = 4,
+    CUSTOS_HIP_KIND_RESTORE8 = 5,
+    CUSTOS_HIP_KIND_UNARY_GRAD8 = 6
 };
 
 /* Allocation flags. */
@@ -437,6 +443,26 @@ enum custos_hip_activation {
 /* Gradients are added to what the operand holds, like custos_hip_add_unary_grad's, unless this is
  * set: then they are stored, so that a first gradient needs no cleared operand and no read of it. */
 #define CUSTOS_HIP_GRAD_OVERWRITE 1
+
+/* 8-bit checkpoints: what a unary operation (or a group norm) needs of its input in the backward pass, in
+ * a quarter or half of its bytes.  128 neighbouring elements share a scale.  With top the largest
+ * finite magnitude of a block: code = x * (127 / top) rounded to the nearest whole number (ties to
+ * even), scale = top * (1 / 127), and the code stands for code * scale, all in f32; so a finite value is
+ * kept to within half a scale.  What is not finite gets code -128, which stands for NaN.  A block
+ * whose top is below 2^-100 is kept as zeros.
+ * `codes`: n bytes; `scales`: ceil(n / 128) f32.  n == 0: nothing is done.
+ *
+ * out[i] = f(x[i]) and the checkpoint of x in one pass; kernel of kind SAVE8.  out 0: only the checkpoint
+ * is made.  out may be x exactly. */
+int32_t custos_hip_checkpoint8_save(custos_hip_device *dev, custos_hip_kernel *kernel, uint64_t x, uint64_t out,
+                                    uint64_t codes, uint64_t scales, size_t n);
+/* out[i] = f(code * scale), rounded once; kernel of kind RESTORE8 (the expression "x" gives the values back). */
+int32_t custos_hip_checkpoint8_restore(custos_hip_device *dev, custos_hip_kernel *kernel, uint64_t codes,
+                                       uint64_t scales, uint64_t out, size_t n);
+/* lhs_grad[i] += out_grad[i] * f(code * scale), rounded like custos_hip_add_unary_grad; kernel of kind
+ * UNARY_GRAD8.  With CUSTOS_HIP_GRAD_OVERWRITE the product is stored, and lhs_grad may be out_grad exactly. */
+int32_t custos_hip_add_unary_grad8(custos_hip_device *dev, custos_hip_kernel *kernel, uint64_t codes,
+                                   uint64_t scales, uint64_t lhs_grad, uint64_t out_grad, size_t n, int32_t flags);
 
 /* x is [samples][positions][channels], `groups` groups of channels / groups neighbouring channels. */
 typedef struct custos_hip_group_norm_desc {

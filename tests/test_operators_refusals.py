@@ -138,3 +138,41 @@ def test_group_norm_formula_against_differences():
                     moved.append(loss(*a))
                 # (error of a central difference: step^2 times a third derivative, and roundings over the step)
                 assert abs((moved[0] - moved[1]) / (2 * step) - grad[at]) < 1e-6, (activation, which, at)
+
+
+# ---- 8-bit checkpoints ----
+
+@pytest.mark.parametrize("kind", [capi.KIND_SAVE8, capi.KIND_RESTORE8, capi.KIND_UNARY_GRAD8])
+def test_checkpoint_kernels_compile_for_the_float_types_and_one_marker(kind):
+    for dtype in ("f32", "f16", "bf16", "f16_pernode", "bf16_pernode"):
+        assert capi.expr_build_code_object(kind, dtype, "pow((x * 2.0), (x + 1.0))", ["x"]) > 1000
+    for dtype in ("f64", "i32", "u8"):
+        with pytest.raises(capi.CustosHipError) as e:
+            capi.expr_emit(kind, dtype, "x", ["x"])
+        assert e.value.code == capi.ERR_EXPR_UNSUPPORTED
+    with pytest.raises(capi.CustosHipError) as e:
+        capi.expr_emit(kind, "f32", "(x + y)", ["x", "y"])
+    assert e.value.code == capi.ERR_ARITY_MISMATCH
+
+
+def test_unknown_kinds_are_refused():
+    for kind in (2, 3, 7, -1):
+        with pytest.raises(capi.CustosHipError, match="unknown kernel kind"):
+            capi.expr_emit(kind, "f32", "x", ["x"])
+
+
+def test_checkpoint_entry_points_refuse_a_missing_kernel():
+    lib = capi.load_library()
+    refused(lib.custos_hip_checkpoint8_save(None, None, BASE, 0, BASE, BASE, 8), INVALID, "null kernel")
+    refused(lib.custos_hip_checkpoint8_restore(None, None, BASE, BASE, BASE, 8), INVALID, "null kernel")
+    refused(lib.custos_hip_add_unary_grad8(None, None, BASE, BASE, BASE, BASE, 8, 0), INVALID, "null kernel")
+
+
+def test_checkpoint_formula():
+    """Half a scale at most, zeros and the largest magnitude exactly at the ends of the code range."""
+    import operator_refs as refs
+    rng = np.random.default_rng(1)
+    x = rng.normal(size=1000).astype(np.float32)
+    codes, scales = refs.checkpoint8(x)
+    assert codes.min() >= -127 and np.abs(codes).max() == 127
+    assert np.all(np.abs(refs.restore8(codes, scales) - x) <= np.repeat(scales, 128)[:1000] * np.float32(0.50001))
