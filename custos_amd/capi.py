@@ -95,6 +95,23 @@ class GroupNormDesc(C.Structure):
     ]
 
 
+class PolicyDesc(C.Structure):
+    """custos_hip_policy_desc"""
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+        ("rows", C.c_uint64),
+        ("vocab", C.c_uint64),
+        ("pitch", C.c_uint64),
+        ("grad_pitch", C.c_uint64),
+        ("temperature", C.c_double),
+        ("clip_low", C.c_double),
+        ("clip_high", C.c_double),
+        ("kl_coef", C.c_double),
+        ("grad_scale", C.c_double),
+    ]
+
+
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 GRAD_OVERWRITE = 1
 
@@ -193,6 +210,8 @@ PROTOTYPES = {
     "custos_hip_add_unary_grad8": (C.c_int32, [_P, _P] + [C.c_uint64] * 4 + [C.c_size_t, C.c_int32]),
     "custos_hip_group_norm": (C.c_int32, [_P, C.POINTER(GroupNormDesc)] + [C.c_uint64] * 7),
     "custos_hip_add_group_norm_grad": (C.c_int32, [_P, C.POINTER(GroupNormDesc)] + [C.c_uint64] * 13),
+    "custos_hip_token_logprob": (C.c_int32, [_P, C.c_int32] + [C.c_uint64] * 5 + [C.c_double] + [C.c_uint64] * 2),
+    "custos_hip_policy_loss": (C.c_int32, [_P, C.POINTER(PolicyDesc)] + [C.c_uint64] * 9),
     "custos_hip_timer_begin": (C.c_int32, [_P]),
     "custos_hip_timer_end": (C.c_int32, [_P, C.POINTER(C.c_double)]),
     "custos_hip_timer_mark": (C.c_int32, [_P, C.c_uint32]),

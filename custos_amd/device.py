@@ -464,6 +464,54 @@ class HIP:
             gamma.ptr if gamma is not None else 0, beta.ptr if beta is not None else 0, out_grad.ptr, out_grad_pitch, x_grad.ptr if x_grad is not None else 0, x_grad_pitch,
             gamma_grad.ptr if gamma_grad is not None else 0, beta_grad.ptr if beta_grad is not None else 0))
 
+    def token_logprob(self, logits: Buffer, labels: Buffer, shape, temperature: float = 1.0, pitch: int | None = None,
+                      out: Buffer | None = None, lse: Buffer | None = None) -> Buffer:
+        """Log-probabilities (f32) of the chosen tokens of `shape` = (rows, vocab) logits, with `lse` also the
+        log of every row's sum (`custos_hip_token_logprob`); labels are i32, a negative one chooses nothing."""
+        rows, vocab = shape
+        pitch = vocab if pitch is None else pitch
+        _holds("logits", logits, _rows_len(rows, vocab, pitch), logits.dtype)
+        _holds("labels", labels, rows, "i32")
+        if out is None:
+            out = self.alloc(rows, "f32", zeroed=False)
+        _holds("out", out, rows, "f32")
+        _holds("lse", lse, rows, "f32")
+        self._check(self.lib.custos_hip_token_logprob(self.handle, capi.DTYPES[logits.dtype][0], logits.ptr, pitch, labels.ptr, rows, vocab,
+                                                      temperature, out.ptr, lse.ptr if lse is not None else 0))
+        return out
+
+    def policy_loss(self, logits: Buffer, labels: Buffer, old_logp: Buffer, advantages: Buffer, weights: Buffer, shape,
+                    ref_logp: Buffer | None = None, clip=(0.2, 0.2), kl_coef: float = 0.0, temperature: float = 1.0,
+                    pitch: int | None = None, logits_grad: Buffer | bool = True, grad_pitch: int | None = None,
+                    grad_scale: float = 1.0, logp: Buffer | None = None, totals: Buffer | None = None):
+        """Clipped policy loss with a KL term over the chosen tokens of `shape` = (rows, vocab) logits, and its
+        gradient (`custos_hip_policy_loss`).  Returns (totals, logp, logits_grad): the f32 totals are the loss and
+        the weighted sums of the KL term, of the clipped rows and of the ratios; `logits_grad` is stored, may be
+        `logits` itself, and False computes none."""
+        rows, vocab = shape
+        pitch = vocab if pitch is None else pitch
+        grad_pitch = vocab if grad_pitch is None else grad_pitch
+        if logits_grad is True:
+            logits_grad = self.alloc(_rows_len(rows, vocab, grad_pitch), logits.dtype, zeroed=False)
+        elif logits_grad is False:
+            logits_grad = None
+        if logp is None:
+            logp = self.alloc(rows, "f32", zeroed=False)
+        if totals is None:
+            totals = self.alloc(4, "f32", zeroed=False)
+        _holds("logits", logits, _rows_len(rows, vocab, pitch), logits.dtype)
+        _holds("logits_grad", logits_grad, _rows_len(rows, vocab, grad_pitch), logits.dtype)
+        _holds("labels", labels, rows, "i32")
+        for name, buf in (("old_logp", old_logp), ("advantages", advantages), ("weights", weights), ("ref_logp", ref_logp), ("logp", logp)):
+            _holds(name, buf, rows, "f32")
+        _holds("totals", totals, 4, "f32")
+        desc = capi.PolicyDesc(capi.DTYPES[logits.dtype][0], 0, rows, vocab, pitch, grad_pitch, temperature, clip[0], clip[1], kl_coef,
+                               grad_scale)
+        self._check(self.lib.custos_hip_policy_loss(
+            self.handle, desc, logits.ptr, labels.ptr, old_logp.ptr, ref_logp.ptr if ref_logp is not None else 0, advantages.ptr,
+            weights.ptr, logits_grad.ptr if logits_grad is not None else 0, logp.ptr, totals.ptr))
+        return totals, logp, logits_grad
+
     # -- caller-written kernels (`launch_kernel` / `launch_kernel1d`, src/devices/cuda/cuda_device.rs:85-112) --
     def _source_args(self, args):
         """Buffers pass their device address, ctypes values and numpy scalars pass with their own

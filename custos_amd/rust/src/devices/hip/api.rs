@@ -40,6 +40,12 @@ pub struct HipGroupNormDesc {
     pub dtype: i32, pub param_dtype: i32, pub activation: i32, pub flags: i32, pub samples: u64, pub positions: u64,
     pub channels: u64, pub groups: u64, pub eps: f64,
 }
+/// `custos_hip_policy_desc`
+#[repr(C)]
+pub struct HipPolicyDesc {
+    pub dtype: i32, pub reserved: i32, pub rows: u64, pub vocab: u64, pub pitch: u64, pub grad_pitch: u64,
+    pub temperature: f64, pub clip_low: f64, pub clip_high: f64, pub kl_coef: f64, pub grad_scale: f64,
+}
 pub const ACT_NONE: i32 = 0;
 pub const ACT_RELU: i32 = 1;
 pub const ACT_SILU: i32 = 2;
@@ -144,6 +150,10 @@ extern "C" {
                                           codes: u64, scales: u64, stats: u64, gamma: u64, beta: u64, out_grad: u64,
                                           out_grad_pitch: u64, x_grad: u64, x_grad_pitch: u64, gamma_grad: u64,
                                           beta_grad: u64) -> i32;
+    pub fn custos_hip_token_logprob(dev: *mut HipDeviceHandle, dtype: i32, logits: u64, pitch: u64, labels: u64, rows: u64,
+                                    vocab: u64, temperature: f64, logp: u64, lse: u64) -> i32;
+    pub fn custos_hip_policy_loss(dev: *mut HipDeviceHandle, desc: *const HipPolicyDesc, logits: u64, labels: u64, old_logp: u64,
+                                  ref_logp: u64, advantages: u64, weights: u64, logits_grad: u64, logp: u64, totals: u64) -> i32;
     pub fn custos_hip_capture_begin(dev: *mut HipDeviceHandle) -> i32;
     pub fn custos_hip_capture_end(dev: *mut HipDeviceHandle, graph: *mut *mut HipGraph) -> i32;
     pub fn custos_hip_capture_end_reuse(dev: *mut HipDeviceHandle, previous: *mut HipGraph,

@@ -495,6 +495,39 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device *dev, const custos_hip_
                                        uint64_t out_grad_pitch, uint64_t x_grad, uint64_t x_grad_pitch,
                                        uint64_t gamma_grad, uint64_t beta_grad);
 
+/* Log-probabilities of chosen tokens: of every row of `vocab` logits (f32, f16 or bf16; `pitch` elements
+ * from row to row), lse = log sum exp(z / T) and logp = z[label] / T - lse, f32 [rows] each; labels are
+ * int32.  A negative label chooses nothing: its logp is 0, and without `lse` (0: not wanted) its row is
+ * not read.  A label behind the vocabulary gives NaN.  Logits of -inf are tokens that cannot be chosen; a
+ * row of nothing else has no distribution: lse -inf, logp NaN.  A row of the type's lowest value
+ * is a uniform one. */
+int32_t custos_hip_token_logprob(custos_hip_device *dev, int32_t dtype, uint64_t logits, uint64_t pitch, uint64_t labels,
+                                 uint64_t rows, uint64_t vocab, double temperature, uint64_t logp, uint64_t lse);
+
+typedef struct custos_hip_policy_desc {
+    int32_t dtype;       /* of the logits and their gradient: CUSTOS_HIP_F32, _F16 or _BF16 */
+    int32_t reserved;    /* 0 */
+    uint64_t rows, vocab, pitch, grad_pitch;
+    double temperature;
+    double clip_low;     /* the ratio is clipped to 1 - clip_low .. 1 + clip_high */
+    double clip_high;
+    double kl_coef;
+    double grad_scale;   /* what the gradient is multiplied by (a loss scale; 1: the gradient itself) */
+} custos_hip_policy_desc;
+
+/* Clipped policy loss with a KL term over chosen tokens, and its gradient to the logits.  With logp as
+ * above, r = exp(logp - old_logp), d = ref_logp - logp and kl = exp(d) - 1 - d, the loss is the sum over
+ * rows of weight * (kl_coef * kl - min(r * advantage, clamp(r) * advantage)).  old_logp,
+ * ref_logp (0: no KL term; kl_coef is 0 then), advantages and weights are f32 [rows]; weights hold the mask
+ * and the normalisation (1 / tokens, or what a mean per sequence asks for).  A row with a negative
+ * label or weight 0 is not read: its logp is 0, its gradient zeros, whatever the row holds.
+ * `logits_grad` (0: not wanted; may be the logits exactly) is stored, not added to; `logp` (0: not
+ * wanted) f32 [rows]; `totals` (0: not wanted) f32 [4]: the loss, and the weighted sums of kl, of the rows
+ * whose clipped term is the smaller one, and of r.  No rows: the totals are zeros. */
+int32_t custos_hip_policy_loss(custos_hip_device *dev, const custos_hip_policy_desc *desc, uint64_t logits,
+                               uint64_t labels, uint64_t old_logp, uint64_t ref_logp, uint64_t advantages,
+                               uint64_t weights, uint64_t logits_grad, uint64_t logp, uint64_t totals);
+
 /* ---- lazy run: capture once, replay (src/devices/cuda/lazy.rs:10-72) ---- */
 
 /* LazySetup::lazy_setup: from here on launches/clears/copies are recorded, not run.

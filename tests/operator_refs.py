@@ -139,3 +139,41 @@ def restore8(codes, scales):
     """The f32 values codes and scales stand for."""
     v = codes.astype(np.float32) * np.repeat(scales, 128)[:codes.size]
     return np.where(codes == -128, np.float32(np.nan), v).astype(np.float32)
+
+
+# ---- log-probabilities and the policy loss ----
+
+def token_logprob(z, labels, temperature):
+    """(logp, lse, softmax) of rows of logits; a negative label's logp is 0, one behind the vocabulary NaN."""
+    z = z / temperature
+    with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
+        top = z.max(1, keepdims=True)
+        e = np.exp(z - np.where(np.isfinite(top), top, 0))
+        total = e.sum(1)
+        lse = top[:, 0] + np.log(total)
+        p = e / total[:, None]
+        at = np.clip(labels, 0, z.shape[1] - 1)
+        logp = np.where(labels < 0, 0.0, np.where(labels >= z.shape[1], np.nan, z[np.arange(len(labels)), at] - lse))
+    return logp, lse, p
+
+
+def policy_loss(z, labels, old, ref, advantage, weight, temperature, clip, kl_coef, grad_scale=1.0):
+    """(totals, logp, gradient) and the magnitude of the gradient's terms at the label and elsewhere."""
+    logp, _, p = token_logprob(z, labels, temperature)
+    used = (labels >= 0) & (weight != 0)
+    logp = np.where(used, logp, 0.0)
+    r = np.exp(logp - old)
+    bounded = np.clip(r, 1 - clip[0], 1 + clip[1])
+    inside = r * advantage <= bounded * advantage
+    d = ref - logp if ref is not None else np.zeros_like(logp)
+    kl = np.expm1(d) - d
+    w = np.where(used, weight, 0.0)
+    totals = np.array([(w * (kl_coef * kl - np.minimum(r * advantage, bounded * advantage))).sum(), (w * kl).sum(), (w * ~inside).sum(), (w * r).sum()])
+    slope = w * (np.where(inside, -advantage * r, 0.0) - kl_coef * np.expm1(d)) * grad_scale / temperature
+    onehot = np.zeros_like(z)
+    onehot[np.arange(len(labels)), np.clip(labels, 0, z.shape[1] - 1)] = 1
+    grad = np.where(used[:, None], slope[:, None] * (onehot - p), 0.0)
+    size = np.abs(w) * (np.abs(advantage) * r + abs(kl_coef) * (np.exp(d) + 1)) * abs(grad_scale) / temperature
+    total_size = np.array([(np.abs(w) * (abs(kl_coef) * (kl + np.abs(d) + 1) + np.abs(advantage) * r)).sum(), (np.abs(w) * (kl + np.abs(d) + 1)).sum(),
+                           np.abs(w).sum(), (np.abs(w) * r).sum()])
+    return totals, logp, grad, np.where(used[:, None], size[:, None] * (onehot + p), 0.0), total_size

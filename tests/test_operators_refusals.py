@@ -176,3 +176,85 @@ def test_checkpoint_formula():
     codes, scales = refs.checkpoint8(x)
     assert codes.min() >= -127 and np.abs(codes).max() == 127
     assert np.all(np.abs(refs.restore8(codes, scales) - x) <= np.repeat(scales, 128)[:1000] * np.float32(0.50001))
+
+
+# ---- log-probabilities and the policy loss ----
+
+def logprob(dtype=F32, logits=BASE, pitch=10, labels=BASE + 0x10000, rows=4, vocab=10, temperature=1.0, logp=BASE + 0x20000, lse=0):
+    return capi.load_library().custos_hip_token_logprob(None, dtype, logits, pitch, labels, rows, vocab, temperature, logp, lse)
+
+
+def policy(over=None, **args):
+    d = dict(dtype=F32, reserved=0, rows=4, vocab=10, pitch=10, grad_pitch=10, temperature=1.0, clip_low=0.2, clip_high=0.2, kl_coef=0.0, grad_scale=1.0)
+    a = dict(logits=BASE, labels=BASE + 0x10000, old_logp=BASE + 0x20000, ref_logp=0, advantages=BASE + 0x30000, weights=BASE + 0x40000,
+             logits_grad=BASE + 0x50000, logp=BASE + 0x60000, totals=BASE + 0x70000)
+    a.update(args)
+    return capi.load_library().custos_hip_policy_loss(None, capi.PolicyDesc(**{**d, **(over or {})}), *a.values())
+
+
+def test_policy_calls_that_pass_every_check_need_a_device():
+    for rc in (logprob(), logprob(lse=BASE + 0x30000), logprob(rows=0), policy(), policy(dict(rows=0)), policy(logits_grad=BASE),
+               policy(dict(kl_coef=0.1), ref_logp=BASE + 0x80000), policy(logits_grad=0, logp=0, totals=0),
+               policy(dict(pitch=20, grad_pitch=20), logits_grad=BASE + 40)):
+        assert rc == INVALID and "device handle is null" in capi.last_error(None)
+        refused(rc, INVALID, "device handle is null")
+
+
+@pytest.mark.parametrize("over, code, text", [
+    (dict(dtype=I32), INVALID, "f32, f16 or bf16"),
+    (dict(vocab=0), INVALID, "vocabulary is empty"),
+    (dict(temperature=0.0), INVALID, "temperature is positive"),
+    (dict(temperature=-1.0), INVALID, "temperature is positive"),
+    (dict(temperature=float("nan")), INVALID, "temperature is positive"),
+    (dict(temperature=float("inf")), INVALID, "temperature is positive"),
+    (dict(temperature=1e-320), INVALID, "temperature is positive"),
+    (dict(temperature=1e300), INVALID, "temperature is positive"),
+    (dict(rows=1 << 31), LARGE, "2^31 rows"),
+    (dict(vocab=1 << 30, pitch=1 << 30), LARGE, "2^30 tokens"),
+    (dict(pitch=9), INVALID, "pitch shorter"),
+])
+def test_rows_of_logits(over, code, text):
+    refused(logprob(**over), code, text)
+    refused(policy(over), code, text)
+
+
+@pytest.mark.parametrize("over, args, code, text", [
+    (dict(reserved=1), {}, INVALID, "reserved"),
+    (dict(clip_low=-0.1), {}, INVALID, "clip_low"),
+    (dict(clip_low=1.5), {}, INVALID, "clip_low"),
+    (dict(clip_high=-0.1), {}, INVALID, "clip_high"),
+    (dict(clip_high=float("nan")), {}, INVALID, "clip_high"),
+    (dict(kl_coef=float("inf")), {}, INVALID, "finite"),
+    (dict(grad_scale=float("nan")), {}, INVALID, "finite"),
+    (dict(kl_coef=0.1), {}, INVALID, "needs ref_logp"),
+    (dict(grad_pitch=3), {}, INVALID, "pitch shorter"),
+    ({}, dict(logits=0), INVALID, "logits is a null"),
+    ({}, dict(labels=0), INVALID, "labels is a null"),
+    ({}, dict(old_logp=0), INVALID, "old_logp is a null"),
+    ({}, dict(advantages=0), INVALID, "advantages is a null"),
+    ({}, dict(weights=0), INVALID, "weights is a null"),
+    ({}, dict(labels=BASE + 2), INVALID, "labels is not aligned"),
+    ({}, dict(logits_grad=BASE + 4), OVERLAP, "overlaps logits"),
+    ({}, dict(logp=BASE), OVERLAP, "logp overlaps logits"),
+    ({}, dict(logp=BASE + 0x20000), OVERLAP, "overlaps"),
+    ({}, dict(totals=BASE + 0x60000), OVERLAP, "overlaps"),
+    ({}, dict(totals=BASE + 0x40000), OVERLAP, "overlaps"),
+])
+def test_policy_refusals(over, args, code, text):
+    refused(policy(over, **args), code, text)
+
+
+def test_policy_formula_against_differences():
+    import operator_refs as refs
+    rng = np.random.default_rng(2)
+    z, labels = rng.normal(size=(8, 6)), rng.integers(0, 6, 8)
+    logp = refs.token_logprob(z, labels, 0.8)[0]
+    old, ref = logp - np.log(rng.choice([0.6, 0.9, 1.1, 1.6], 8)), logp + 0.3 * rng.normal(size=8)
+    adv, w = rng.normal(size=8), rng.random(8)
+    args = (labels, old, ref, adv, w, 0.8, (0.2, 0.3), 0.2)
+    grad = refs.policy_loss(z, *args)[2]
+    for at in np.ndindex(z.shape):
+        up, down = z.copy(), z.copy()
+        up[at] += 1e-5
+        down[at] -= 1e-5
+        assert abs((refs.policy_loss(up, *args)[0][0] - refs.policy_loss(down, *args)[0][0]) / 2e-5 - grad[at]) < 1e-7, at
