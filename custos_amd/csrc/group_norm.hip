@@ -27,10 +27,27 @@ namespace custos_hip {
 namespace {
 
 constexpr int kBlock = 256;      // threads of the kernels that stream
-constexpr int kMaxTileGroups = 64;  // groups per tile of the kernels that hold a tile in registers
-constexpr int kMaxStreamGroups = 2048;  // groups per tile of the kernels that stream (kBlock vectors of 8 channels)
+constexpr int kMaxTileGroups = 64;     // groups per tile of the kernels that hold a tile in registers
+constexpr int kMaxStreamGroups = 128;  // groups per tile of the kernels that stream
 
 enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
+
+// Division of 32-bit numbers by one the host knows.
+struct Divisor {
+    unsigned int by = 1, magic = 0;  // floor(2^32 / by); by == 1: 0, and the correction below gives the answer
+    __device__ __forceinline__ unsigned int divide(unsigned int n) const {
+        if (by == 1) return n;
+        unsigned int q = __umulhi(n, magic);  // (at most one too small)
+        return n - q * by >= by ? q + 1 : q;
+    }
+};
+// How the rows of a sample are dealt out to workgroups: `rounds` rounds of `step` rows each, to the first `longer` of
+// them one more.
+struct Splits {
+    unsigned int count = 1, longer = 0;
+    u64 rounds = 0;
+    Divisor by_count;
+};
 
 struct GroupNormArgs {
     const void* x;            // or null: codes and scales of an 8-bit checkpoint
@@ -41,13 +58,28 @@ struct GroupNormArgs {
     const void* out_grad;     // backward
     void* out;                // out, or x_grad
     float* stats;             // [samples][groups]: mean, rstd
-    float* partial;           // work area
-    float* sums;              // backward, work area: [samples][groups] pairs
-    u64 positions, rows;      // rows: positions a workgroup of a streaming kernel takes
+    // Work area, a "part" being the positions of a sample that one workgroup of the first pass takes (all of them for
+    // a tile in registers).  Forward: [samples][parts][groups] pairs of a mean and a sum of squared
+    // distances.  Backward: the same of the sums of dz * gamma and of dz * gamma * h, and `channel_parts`.
+    float* group_parts;
+    float* channel_parts;     // [samples][parts][2][channels]: sums of dz and of dz * h
+    float* gamma_grad;
+    float* beta_grad;
+    u64 positions;
     u64 x_pitch, grad_pitch, out_pitch;
-    unsigned int samples, channels, groups, per_group, tile_groups, tiles, splits;
+    unsigned int samples, channels, groups, per_group, tile_groups, tiles;
+    Splits parts, values;          // of the first pass (a part each), and of the second
+    Divisor by_tiles;
+    unsigned int vecs, vecs_magic; // vectors per row of a tile; ceil(2^32 / vecs)
+    unsigned int waves_per_group, waves_magic;  // where a tile has fewer groups than a workgroup has wavefronts
+    double total_inverse;          // 1 / values of a group
+    int whole_groups;              // no vector of a row has channels of two groups
+    unsigned int step;             // rows a workgroup of a streaming kernel reads at a time
+    unsigned int part_step;        // the first pass's
+    unsigned int last_part, missing_rows;  // the part with the last round of rows, and how many that is short of `step`
+    unsigned int blocks;           // workgroups that work on values; what follows them adds up gamma_grad and beta_grad
     unsigned int per_group_magic;  // ceil(2^32 / per_group), for divisions of numbers below 2^16
-    int param_f32, activation, accumulate;
+    int param_f32, accumulate;
     float eps;
 };
 
@@ -60,6 +92,33 @@ template <class T>
 __device__ __forceinline__ float param(const void* p, int f32, unsigned int i, float none) {
     if (!p) return none;
     return f32 ? static_cast<const float*>(p)[i] : to_f32(static_cast<const T*>(p)[i]);
+}
+
+// V of them, with one branch and wide loads.
+template <class T, int V>
+__device__ __forceinline__ void params(const void* p, int f32, unsigned int first, float none, float (&out)[V]) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < V; j++) out[j] = none;
+    } else if (f32) {
+        constexpr int W = V >= 4 ? 4 : 1;
+#pragma unroll
+        for (int j = 0; j < V; j += W) {
+            const Pack<float, W> v = load_pack<false, float, W>(static_cast<const float*>(p) + first + j);
+#pragma unroll
+            for (int k = 0; k < W; k++) out[j + k] = v.v[k];
+        }
+    } else {
+        const Pack<T, V> v = load_pack<false, T, V>(static_cast<const T*>(p) + first);
+#pragma unroll
+        for (int j = 0; j < V; j++) out[j] = to_f32(v.v[j]);
+    }
+}
+
+// Roundings may leave a sum of squares just below zero; a NaN stays one.
+template <class F>
+__device__ __forceinline__ F not_negative(F v) {
+    return v < F(0) ? F(0) : v;
 }
 
 // exp(-z) through the hardware exp2: relative error below |z| 2^-24 + 1 ulp.
@@ -78,25 +137,16 @@ __device__ __forceinline__ float act_grad(float z) {
     if (ACT == kRelu) return z > 0.0f ? 1.0f : 0.0f;
     if (ACT == kSilu) {
         const float s = sigmoid(z);
-        return s * (1.0f + z * (1.0f - s));
+        return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
     }
     if (ACT == kGelu)
         return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * (0.39894228f * __builtin_amdgcn_exp2f(z * z * -0.72134752f));
     return 1.0f;
 }
-template <class F>
-__device__ __forceinline__ void with_activation(int activation, F f) {
-    switch (activation) {
-        case kRelu: f(std::integral_constant<int, kRelu>()); break;
-        case kSilu: f(std::integral_constant<int, kSilu>()); break;
-        case kGelu: f(std::integral_constant<int, kGelu>()); break;
-        default: f(std::integral_constant<int, kNone>()); break;
-    }
-}
-
 // Which part of the data a thread of a tile works on: a vector of V channels, the same for all its rows.
 // The last vector of a row of W channels starts at W - V; its first `dup` channels are also the vector
-// before it's: loaded, but neither summed nor stored here.
+// before it's: they are not summed here, and stored by both with the same value (where that would not do, rows are
+// worked on channel by channel: narrow_values).
 struct Column {
     unsigned int width;   // channels of the tile
     unsigned int vecs;    // vectors per row
@@ -120,92 +170,96 @@ __device__ __forceinline__ Column column_of(const GroupNormArgs& a, unsigned int
 // x as the kernels read it: V elements of T, or of an 8-bit checkpoint.
 template <class T, int V, bool SAVED>
 struct Source {
-    Pack<T, V> p;
+    Bits<T, V> p;
+    template <bool STREAM = false>
     __device__ __forceinline__ void load(const GroupNormArgs& a, u64 row, unsigned int channel) {
-        p = load_pack<false, T, V>(static_cast<const T*>(a.x) + row * a.x_pitch + channel);
+        p.template load<STREAM>(static_cast<const T*>(a.x) + row * a.x_pitch + channel);
     }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int j = 0; j < V; j++) p.v[j] = from_f32<T>(0.0f);
-    }
-    __device__ __forceinline__ float value(int j) const { return to_f32(p.v[j]); }
+    __device__ __forceinline__ void zero() { p.zero(); }
+    __device__ __forceinline__ void forget_values() { p.forget_values(); }
+    __device__ __forceinline__ float value(int j) const { return to_f32(p.pack().v[j]); }
 };
 template <class T, int V>
 struct Source<T, V, true> {
-    Pack<signed char, V> c;
+    Bits<signed char, V> c;
     float low, high;  // the vector may end in the next block of 128
     int in_low;
+    template <bool STREAM = false>
     __device__ __forceinline__ void load(const GroupNormArgs& a, u64 row, unsigned int channel) {
         const u64 i = row * a.channels + channel;
-        c = load_pack<false, signed char, V>(a.codes + i);
+        c.template load<STREAM>(a.codes + i);
         in_low = 128 - static_cast<int>(i & 127);
         low = a.scales[i >> 7];
         high = in_low < V ? a.scales[(i >> 7) + 1] : low;
     }
     __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int j = 0; j < V; j++) c.v[j] = 0;
+        c.zero();
         low = high = 0.0f;
         in_low = V;
     }
+    __device__ __forceinline__ void forget_values() { c.forget_values(); }
     __device__ __forceinline__ float value(int j) const {
-        const float v = static_cast<float>(c.v[j]) * (j < in_low ? low : high);
-        return c.v[j] == -128 ? __builtin_nanf("") : v;
+        const signed char code = c.pack().v[j];
+        const float v = static_cast<float>(code) * (j < in_low ? low : high);
+        return code == -128 ? __builtin_nanf("") : v;
     }
 };
 
-template <class T, int V>
-__device__ __forceinline__ void store_valid(T* p, const Pack<T, V>& pack, int dup) {
-    if (dup == 0) {
-        store_pack<false, T, V>(p, pack);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; j++)
-            if (j >= dup) p[j] = pack.v[j];
-    }
-}
+// How many values every channel of row `r` of a workgroup's threads stands for: `rounds`, one less from row `whole` on.
+struct RowCounts {
+    float rounds;
+    unsigned int whole;
+    __device__ __forceinline__ float of(unsigned int r) const { return r < whole ? rounds : rounds - 1.0f; }
+};
 
-// Sums of a table of `rows` x `width` floats over the rows and channels of each group; result for group g in
-// out[g].  All threads of the workgroup call it; `table` is complete when it is called and free when it
-// returns, `out` may be read then.
+// Mean and sum of squared distances of every group of a tile, from those of `step` x `width` channels (`table`):
+// in f64, about the first entry's mean, so that no large numbers cancel.  All threads of the workgroup call it;
+// result for group g in out[g], to be read after the return.
 template <int THREADS>
-__device__ __forceinline__ void group_sums(const float* table, unsigned int rows, unsigned int width, unsigned int n_groups,
-                                           unsigned int per_group, unsigned int magic, float* wave_sums, float* out) {
+__device__ __forceinline__ void merge_groups(const GroupNormArgs& a, const float2* table, const RowCounts& counts, float total_inverse, float2* out) {
     constexpr unsigned int kWaves = THREADS / 64;
-    const unsigned int t = threadIdx.x, entries = rows * per_group;
+    __shared__ double wave_sums[kWaves][2];
+    const unsigned int t = threadIdx.x, width = a.tile_groups * a.per_group, entries = a.step * a.per_group;
+    const bool shared = a.tile_groups < kWaves;  // several wavefronts per group, else several groups per wavefront
+    unsigned int per = kWaves, lanes = 64;
+    if (shared) per = a.waves_per_group;
+    else
+        while (lanes > 1 && lanes * a.tile_groups > static_cast<unsigned int>(THREADS)) lanes /= 2;
     __syncthreads();
-    if (n_groups < kWaves) {
-        // several wavefronts per group
-        const unsigned int per = kWaves / n_groups, wave = t / 64, g = wave / per;
-        float s = 0.0f;
-        if (g < n_groups)
-            for (unsigned int e = (wave % per) * 64 + t % 64; e < entries; e += per * 64) {
-                const unsigned int r = group_of(e, magic);
-                s += table[r * width + g * per_group + (e - r * per_group)];
+    for (unsigned int base = 0; base < a.tile_groups; base += THREADS / lanes) {
+        const unsigned int wave = t / 64, g = shared ? group_of(wave, a.waves_magic) : base + t / lanes;
+        const unsigned int begin = shared ? (wave - g * per) * 64 + t % 64 : t % lanes, by = shared ? per * 64 : lanes;
+        double first = 0.0, second = 0.0;
+        float about = 0.0f;
+        if (g < a.tile_groups) {
+            about = table[g * a.per_group].x;
+            for (unsigned int e = begin; e < entries; e += by) {
+                const unsigned int r = group_of(e, a.per_group_magic);
+                const float2 v = table[r * width + g * a.per_group + (e - r * a.per_group)];
+                const double count = counts.of(r), d = v.x - about;
+                first += count * d;
+                second += v.y + count * d * d;
             }
-        s = lanes_sum<64>(s);
-        if (t % 64 == 0) wave_sums[wave] = s;
-        __syncthreads();
-        if (t < n_groups) {
-            float total = 0.0f;
-            for (unsigned int i = 0; i < per; i++) total += wave_sums[t * per + i];
-            out[t] = total;
         }
-    } else {
-        // several groups per wavefront: a power of two of lanes for each
-        int lanes = 64;
-        while (static_cast<unsigned int>(lanes) * n_groups > THREADS && lanes > 1) lanes /= 2;
-        for (unsigned int base = 0; base < n_groups; base += THREADS / lanes) {
-            const unsigned int g = base + t / lanes;
-            float s = 0.0f;
-            if (g < n_groups)
-                for (unsigned int e = t % lanes; e < entries; e += lanes) {
-                    const unsigned int r = group_of(e, magic);
-                    s += table[r * width + g * per_group + (e - r * per_group)];
-                }
-            s = lanes_sum_of(s, lanes);
-            if (g < n_groups && t % lanes == 0) out[g] = s;
+        for (unsigned int half = lanes / 2; half > 0; half /= 2) {
+            first += __shfl_xor(first, half, 64);
+            second += __shfl_xor(second, half, 64);
         }
+        if (shared) {
+            if (t % 64 == 0) wave_sums[wave][0] = first, wave_sums[wave][1] = second;
+            __syncthreads();
+            first = second = 0.0;
+            if (t < a.tile_groups) {
+                about = table[t * a.per_group].x;
+                for (unsigned int i = 0; i < per; i++) first += wave_sums[t * per + i][0], second += wave_sums[t * per + i][1];
+            }
+        }
+        const unsigned int mine = shared ? t : g;
+        if (mine < a.tile_groups && (shared || t % lanes == 0)) {
+            const double mean = first * total_inverse;
+            out[mine] = make_float2(static_cast<float>(about + mean), static_cast<float>(not_negative(second - first * mean)));
+        }
+        if (shared) break;
     }
     __syncthreads();
 }
@@ -223,214 +277,321 @@ __device__ __forceinline__ float block_sum(float v, float* wave_sums) {
     return total;
 }
 
-// ---- forward, a tile in registers: one launch, x read once ----
+// The rows of a tile that one workgroup of a streaming kernel works on, and its threads' shares.  The workgroups of a
+// sample take turns, `step` rows at a time, so that those that run together read neighbouring memory (each on a
+// stretch of its own, at equal distances, they would meet in the same memory channels).
+template <int V>
+struct Stream {
+    unsigned int n, part, tile, c0, vecs, step, r0, col0;
+    u64 first, stride, rows;  // the thread's first row (of all samples), from row to row, and how many rows it has
+    bool one_column;          // else a thread has several columns and every row
+    __device__ __forceinline__ Stream(const GroupNormArgs& a, const Splits& of, unsigned int index) {
+        const unsigned int t = threadIdx.x;
+        const unsigned int block = a.by_tiles.divide(index);
+        tile = index - block * a.tiles;
+        const unsigned int sample = of.by_count.divide(block), split = block - sample * of.count;
+        n = sample;
+        part = block;
+        vecs = a.vecs;
+        one_column = vecs <= kBlock;
+        step = a.step;
+        r0 = one_column ? group_of(t, a.vecs_magic) : 0;
+        col0 = one_column ? t - r0 * vecs : t;
+        stride = static_cast<u64>(of.count) * step;
+        const u64 p = static_cast<u64>(split) * step + r0;
+        first = static_cast<u64>(n) * a.positions + p;
+        rows = of.rounds + (split < of.longer ? 1 : 0);
+        if (r0 >= step) rows = 0;
+        else if (rows > 0 && p + (rows - 1) * stride >= a.positions) rows--;
+        c0 = tile * a.tile_groups * a.per_group;
+    }
+    __device__ __forceinline__ bool active() const { return r0 < step; }
+};
 
-template <class T, int V, int HELD, int THREADS>
-__global__ void __launch_bounds__(THREADS) custos_group_norm_tile(const GroupNormArgs a) {
-    __shared__ float table[THREADS * V];
-    __shared__ float wave_sums[THREADS / 64];
-    __shared__ float mean_of[kMaxTileGroups], rstd_of[kMaxTileGroups];
-    const unsigned int t = threadIdx.x;
-    const unsigned int n = blockIdx.x / a.tiles, tile = blockIdx.x - n * a.tiles;
-    const unsigned int vecs = (a.tile_groups * a.per_group + V - 1) / V;
-    const unsigned int step = THREADS / vecs;  // rows at a time (the host made sure that it is at least one)
-    const unsigned int r0 = t / vecs;
-    const Column c = column_of<V>(a, t - r0 * vecs);
-    const bool active = r0 < step;
-    const unsigned int c0 = tile * a.tile_groups * a.per_group;
-    const u64 row0 = static_cast<u64>(n) * a.positions;
-    Source<T, V, false> held[HELD];
-#pragma unroll
-    for (int i = 0; i < HELD; i++) {
-        const u64 p = r0 + static_cast<u64>(i) * step;
-        if (active && p < a.positions) held[i].load(a, row0 + p, c0 + c.first);
-        else held[i].zero();
-    }
-    const float count = static_cast<float>(a.positions) * static_cast<float>(a.per_group);
-    float sum[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        sum[j] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HELD; i++) sum[j] += held[i].value(j);
-        if (active && j >= c.dup) table[r0 * c.width + c.first + j] = sum[j];
-    }
-    group_sums<THREADS>(table, step, c.width, a.tile_groups, a.per_group, a.per_group_magic, wave_sums, mean_of);
-    float mean[V], rstd[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) mean[j] = mean_of[group_of(c.first + j, a.per_group_magic)] / count;
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        sum[j] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HELD; i++) {
-            const float d = held[i].value(j) - mean[j];
-            if (r0 + static_cast<u64>(i) * step < a.positions) sum[j] += d * d;
-        }
-        if (active && j >= c.dup) table[r0 * c.width + c.first + j] = sum[j];
-    }
-    group_sums<THREADS>(table, step, c.width, a.tile_groups, a.per_group, a.per_group_magic, wave_sums, rstd_of);
-#pragma unroll
-    for (int j = 0; j < V; j++) rstd[j] = 1.0f / sqrtf(rstd_of[group_of(c.first + j, a.per_group_magic)] / count + a.eps);
-    if (t < a.tile_groups) {
-        float* s = a.stats + (static_cast<u64>(n) * a.groups + tile * a.tile_groups + t) * 2;
-        s[0] = mean_of[t] / count;
-        s[1] = 1.0f / sqrtf(rstd_of[t] / count + a.eps);
-    }
-    if (!active) return;
-    float gamma[V], beta[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        gamma[j] = param<T>(a.gamma, a.param_f32, c0 + c.first + j, 1.0f);
-        beta[j] = param<T>(a.beta, a.param_f32, c0 + c.first + j, 0.0f);
-    }
-    T* out = static_cast<T*>(a.out) + row0 * a.out_pitch + c0 + c.first;
-    with_activation(a.activation, [&](auto which) {
-#pragma unroll
-        for (int i = 0; i < HELD; i++) {
-            const u64 p = r0 + static_cast<u64>(i) * step;
-            if (p >= a.positions) break;
-            Pack<T, V> y;
-#pragma unroll
-            for (int j = 0; j < V; j++)
-                y.v[j] = from_f32<T>(act<decltype(which)::value>((held[i].value(j) - mean[j]) * rstd[j] * gamma[j] + beta[j]));
-            store_valid<T, V>(out + p * a.out_pitch, y, c.dup);
-        }
-    });
+// Positions of part `split` of a sample.
+__device__ __forceinline__ u64 part_rows(const GroupNormArgs& a, unsigned int split) {
+    return (a.parts.rounds + (split < a.parts.longer ? 1 : 0)) * a.part_step - (split == a.last_part ? a.missing_rows : 0);
 }
 
-// ---- forward, streaming: parts of every group, the parts joined, the values ----
+// Workgroups are dealt to the eight XCDs in turn, each with an L2 of its own.  This order gives an XCD neighbouring
+// tiles, which share cache lines where a tile's rows are no whole lines.
+__device__ __forceinline__ unsigned int by_xcd(unsigned int block, unsigned int blocks) {
+    return blocks % 8 == 0 ? block % 8 * (blocks / 8) + block / 8 : block;
+}
 
-// Mean and sum of squared distances of every group over the rows of one part.
+// ---- forward, a tile in registers: one launch, x read once ----
+
+template <class T, int V, int HELD, int THREADS, int ACT>
+__global__ void __launch_bounds__(THREADS) custos_group_norm_tile(const GroupNormArgs a) {
+    __shared__ float2 table[THREADS * V];
+    __shared__ float2 stats[kMaxTileGroups];
+    const unsigned int t = threadIdx.x;
+    const unsigned int index = by_xcd(blockIdx.x, gridDim.x), n = a.by_tiles.divide(index), tile = index - n * a.tiles;
+    const unsigned int step = a.step;  // rows at a time
+    const unsigned int r0 = group_of(t, a.vecs_magic);
+    const Column c = column_of<V>(a, t - r0 * a.vecs);
+    const bool active = r0 < step;
+    const unsigned int c0 = tile * a.tile_groups * a.per_group, positions = static_cast<unsigned int>(a.positions);
+    const T* x = static_cast<const T*>(a.x) + (static_cast<u64>(n) * a.positions + r0) * a.x_pitch + c0 + c.first;
+    const unsigned int rounds = active && r0 < positions ? static_cast<unsigned int>(a.parts.rounds) - (r0 + (a.parts.rounds - 1) * step >= positions ? 1 : 0) : 0;
+    Bits<T, V> held[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+        if (static_cast<unsigned int>(i) < rounds) held[i].load(x + static_cast<u64>(i) * step * a.x_pitch);
+    float scale[V], shift[V];  // of the channels: gamma and beta until the statistics are there
+    params<T, V>(a.gamma, a.param_f32, c0 + c.first, 1.0f, scale);
+    params<T, V>(a.beta, a.param_f32, c0 + c.first, 0.0f, shift);
+    // of the thread's channels: mean, then squared distances from it
+    {
+        float mean[V], m2[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) mean[j] = m2[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < HELD; i++) {
+            if (static_cast<unsigned int>(i) >= rounds) break;
+            const Pack<T, V> p = held[i].pack();
+#pragma unroll
+            for (int j = 0; j < V; j++) mean[j] += to_f32(p.v[j]);
+            held[i].forget_values();
+        }
+        const float inverse = rounds > 0 ? 1.0f / static_cast<float>(rounds) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; j++) mean[j] *= inverse;
+#pragma unroll
+        for (int i = 0; i < HELD; i++) {
+            if (static_cast<unsigned int>(i) >= rounds) break;
+            const Pack<T, V> p = held[i].pack();
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float d = to_f32(p.v[j]) - mean[j];
+                m2[j] = __builtin_fmaf(d, d, m2[j]);
+            }
+            held[i].forget_values();
+        }
+        if (active) {
+            float2* row = table + r0 * c.width + c.first;
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (j >= c.dup) row[j] = make_float2(mean[j], m2[j]);
+        }
+    }
+    const float total = static_cast<float>(a.positions) * static_cast<float>(a.per_group), total_inverse = 1.0f / total;
+    const RowCounts counts{static_cast<float>(a.parts.rounds), step - a.missing_rows};
+    merge_groups<THREADS>(a, table, counts, total_inverse, stats);
+    if (t < a.tile_groups) {
+        const float2 s = make_float2(stats[t].x, 1.0f / sqrtf(stats[t].y * total_inverse + a.eps));
+        stats[t] = s;
+        reinterpret_cast<float2*>(a.stats)[static_cast<u64>(n) * a.groups + tile * a.tile_groups + t] = s;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        const float2 s = stats[group_of(c.first + j, a.per_group_magic)];
+        scale[j] *= s.y;
+        shift[j] = __builtin_fmaf(-s.x, scale[j], shift[j]);
+    }
+    T* out = static_cast<T*>(a.out) + (static_cast<u64>(n) * a.positions + r0) * a.out_pitch + c0 + c.first;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        if (static_cast<unsigned int>(i) >= rounds) break;
+        const Pack<T, V> p = held[i].pack();
+        Pack<T, V> y;
+#pragma unroll
+        for (int j = 0; j < V; j++) y.v[j] = from_f32<T>(act<ACT>(__builtin_fmaf(to_f32(p.v[j]), scale[j], shift[j])));
+        store_pack<false, T, V>(out + static_cast<u64>(i) * step * a.out_pitch, y);
+    }
+}
+
+// ---- forward, streaming: parts of every group and their join, then the values ----
+
+// Mean and sum of squared distances of every group over the rows of one part.  A thread sums distances from the
+// first value it meets in each channel.
 template <class T, int V>
 __global__ void __launch_bounds__(kBlock) custos_group_norm_parts(const GroupNormArgs a) {
-    __shared__ float table[kBlock * V];
+    __shared__ float2 table[kBlock * V];
     __shared__ float wave_sums[kBlock / 64];
-    __shared__ float group[kMaxStreamGroups];
+    __shared__ float2 group[kMaxStreamGroups];
     const unsigned int t = threadIdx.x;
-    const unsigned int part = blockIdx.x / a.tiles, tile = blockIdx.x - part * a.tiles;
-    const unsigned int n = part / a.splits, split = part - n * a.splits;
-    const u64 p0 = split * a.rows, p1 = min(p0 + a.rows, a.positions);
-    const unsigned int vecs = (a.tile_groups * a.per_group + V - 1) / V;
-    const bool one_column = vecs <= kBlock;
-    const unsigned int step = one_column ? kBlock / vecs : 1;
-    const unsigned int r0 = one_column ? t / vecs : 0;
-    const unsigned int c0 = tile * a.tile_groups * a.per_group;
-    const u64 row0 = static_cast<u64>(n) * a.positions;
-    const u64 rows = r0 < step && p0 + r0 < p1 ? (p1 - p0 - r0 + step - 1) / step : 0;
-    float* out = a.partial + (static_cast<u64>(part) * a.groups + tile * a.tile_groups) * 2;
+    const Stream<V> w(a, a.parts, blockIdx.x);
+    float2* out = reinterpret_cast<float2*>(a.group_parts) + static_cast<u64>(w.part) * a.groups + w.tile * a.tile_groups;
+    const float rows = static_cast<float>(w.rows);
     // of the thread, over all its columns (one group per tile), or of its column
     float all = 0.0f, all_mean = 0.0f, all_m2 = 0.0f;
     float mean[V], m2[V];
-    Column c = column_of<V>(a, one_column ? t - r0 * vecs : t);
-    for (unsigned int col = one_column ? t - r0 * vecs : t; col < vecs && r0 < step; col += kBlock) {
+    Column c = column_of<V>(a, w.col0);
+    for (unsigned int col = w.col0; col < w.vecs && w.active(); col += kBlock) {
         c = column_of<V>(a, col);
-        const u64 first = row0 + p0 + r0;
+        const unsigned int channel = w.c0 + c.first;
         float shift[V], s[V], q[V];
 #pragma unroll
         for (int j = 0; j < V; j++) shift[j] = s[j] = q[j] = mean[j] = m2[j] = 0.0f;
-        if (rows > 0) {
+        if (w.rows > 0) {
             Source<T, V, false> x;
-            x.load(a, first, c0 + c.first);
+            x.load(a, w.first, channel);
 #pragma unroll
             for (int j = 0; j < V; j++) shift[j] = x.value(j);
         }
-        constexpr int kAhead = 4;
-        u64 i = 0;
-        for (; i + kAhead <= rows; i += kAhead) {
-            Source<T, V, false> x[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) x[u].load(a, first + (i + u) * step, c0 + c.first);
-#pragma unroll
-            for (int u = 0; u < kAhead; u++)
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float d = x[u].value(j) - shift[j];
-                    s[j] += d;
-                    q[j] = __builtin_fmaf(d, d, q[j]);
-                }
-        }
-        for (; i < rows; i++) {
-            Source<T, V, false> x;
-            x.load(a, first + i * step, c0 + c.first);
+        auto add = [&](const Source<T, V, false>& x) {
 #pragma unroll
             for (int j = 0; j < V; j++) {
                 const float d = x.value(j) - shift[j];
                 s[j] += d;
                 q[j] = __builtin_fmaf(d, d, q[j]);
             }
+        };
+        constexpr int kAhead = 4;
+        u64 i = 0;
+        for (; i + kAhead <= w.rows; i += kAhead) {
+            Source<T, V, false> x[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) x[u].load(a, w.first + (i + u) * w.stride, channel);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) add(x[u]);
         }
-        if (rows > 0) {
-            const float count = static_cast<float>(rows);
+        for (; i < w.rows; i++) {
+            Source<T, V, false> x;
+            x.load(a, w.first + i * w.stride, channel);
+            add(x);
+        }
+        if (w.rows > 0) {
+            const float per = 1.0f / rows;
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                mean[j] = shift[j] + s[j] / count;
-                m2[j] = fmaxf(q[j] - s[j] * (s[j] / count), 0.0f);
+                mean[j] = __builtin_fmaf(s[j], per, shift[j]);
+                m2[j] = not_negative(q[j] - s[j] * (s[j] * per));
             }
         }
-        if (a.tile_groups == 1 && rows > 0) {
+        if (a.tile_groups == 1 && w.rows > 0) {
             // the column's channels are one group's: count, mean and squared distances of the thread
-            const float count = static_cast<float>(rows) * static_cast<float>(V - c.dup);
+            const float valid = static_cast<float>(V - c.dup), count = rows * valid;
             float m = 0.0f, d2 = 0.0f;
 #pragma unroll
             for (int j = 0; j < V; j++) m += j >= c.dup ? mean[j] : 0.0f;
-            m /= static_cast<float>(V - c.dup);
+            m /= valid;
 #pragma unroll
             for (int j = 0; j < V; j++)
-                if (j >= c.dup) d2 += m2[j] + static_cast<float>(rows) * (mean[j] - m) * (mean[j] - m);
+                if (j >= c.dup) d2 += m2[j] + rows * (mean[j] - m) * (mean[j] - m);
             const float both = all + count, delta = m - all_mean;
             all_m2 += d2 + delta * delta * (all * (count / both));
             all_mean += delta * (count / both);
             all = both;
         }
     }
-    const float total = static_cast<float>(p1 - p0) * static_cast<float>(a.per_group);
+    const unsigned int split = w.part - w.n * a.parts.count;
+    const float total_inverse = 1.0f / (static_cast<float>(part_rows(a, split)) * static_cast<float>(a.per_group));
     if (a.tile_groups == 1) {
-        const float m = block_sum<kBlock>(all * all_mean, wave_sums) / total;
+        const float m = block_sum<kBlock>(all * all_mean, wave_sums) * total_inverse;
         const float d2 = block_sum<kBlock>(all_m2 + all * (all_mean - m) * (all_mean - m), wave_sums);
-        if (t == 0) out[0] = m, out[1] = d2;
+        if (t == 0) *out = make_float2(m, d2);
         return;
     }
-    const bool active = r0 < step;
+    if (w.active()) {
+        float2* row = table + w.r0 * c.width + c.first;
 #pragma unroll
-    for (int j = 0; j < V; j++)
-        if (active && j >= c.dup) table[r0 * c.width + c.first + j] = static_cast<float>(rows) * mean[j];
-    group_sums<kBlock>(table, step, c.width, a.tile_groups, a.per_group, a.per_group_magic, wave_sums, group);
-    for (unsigned int g = t; g < a.tile_groups; g += kBlock) out[g * 2] = group[g] / total;
-#pragma unroll
-    for (int j = 0; j < V; j++)
-        if (active && j >= c.dup) {
-            const float d = mean[j] - group[group_of(c.first + j, a.per_group_magic)] / total;
-            table[r0 * c.width + c.first + j] = m2[j] + static_cast<float>(rows) * d * d;
-        }
-    __syncthreads();  // (every thread has read `group`)
-    group_sums<kBlock>(table, step, c.width, a.tile_groups, a.per_group, a.per_group_magic, wave_sums, group);
-    for (unsigned int g = t; g < a.tile_groups; g += kBlock) out[g * 2 + 1] = group[g];
+        for (int j = 0; j < V; j++)
+            if (j >= c.dup) row[j] = make_float2(mean[j], m2[j]);
+    }
+    const RowCounts counts{static_cast<float>(a.parts.rounds + (split < a.parts.longer ? 1 : 0)), w.step - (split == a.last_part ? a.missing_rows : 0)};
+    merge_groups<kBlock>(a, table, counts, total_inverse, group);
+    for (unsigned int g = t; g < a.tile_groups; g += kBlock) out[g] = group[g];
 }
 
-// The parts of a group joined, one wavefront for each: lanes over the parts, sums in f64.
-__global__ void __launch_bounds__(kBlock) custos_group_norm_stats(const GroupNormArgs a) {
-    const u64 which = static_cast<u64>(blockIdx.x) * (kBlock / 64) + threadIdx.x / 64;
-    if (which >= static_cast<u64>(a.samples) * a.groups) return;
-    const unsigned int lane = threadIdx.x % 64;
-    const u64 n = which / a.groups, g = which - n * a.groups;
-    const float* part = a.partial + (n * a.splits * a.groups + g) * 2;
-    auto count = [&](unsigned int s) { return static_cast<double>(min(a.rows, a.positions - s * a.rows)) * a.per_group; };
-    double sum = 0.0;
-    for (unsigned int s = lane; s < a.splits; s += 64) sum += count(s) * part[static_cast<u64>(s) * a.groups * 2];
-    const double total = static_cast<double>(a.positions) * a.per_group;
-    const double mean = lanes_sum_f64(sum) / total;
-    double m2 = 0.0;
-    for (unsigned int s = lane; s < a.splits; s += 64) {
-        const double d = part[static_cast<u64>(s) * a.groups * 2] - mean;
-        m2 += part[static_cast<u64>(s) * a.groups * 2 + 1] + count(s) * d * d;
+// The parts of the tile's groups joined, in f64 and in a fixed order.  Every workgroup of the second pass does it for
+// itself: at most 32 KiB, from the L2, against a launch of its own (4 to 5 us), or a last workgroup of the first
+// pass that joins for all (the fences that needs between the L2s of the chip took 100 us of a pass of 80).
+// `of(group, a, b)` receives each group's mean and deviation (FORWARD), or the two means of the gradient.
+template <bool FORWARD, class F>
+__device__ __forceinline__ void join_parts(const GroupNormArgs& a, unsigned int n, unsigned int tile, F of) {
+    __shared__ double sums[2][kBlock];
+    const unsigned int t = threadIdx.x;
+    unsigned int lanes = 1;
+    while (lanes * 2 * a.tile_groups <= static_cast<unsigned int>(kBlock)) lanes *= 2;
+    const unsigned int lane = t / a.tile_groups, g = t - lane * a.tile_groups;
+    const float2* part = reinterpret_cast<const float2*>(a.group_parts) + static_cast<u64>(n) * a.parts.count * a.groups + tile * a.tile_groups + g;
+    double first = 0.0, second = 0.0;
+    // means are taken from that of part 0, which is near all of them
+    const double base = FORWARD ? part[0].x : 0.0;
+    if (lane < lanes)
+        for (unsigned int s = lane; s < a.parts.count; s += lanes) {
+            const float2 v = part[static_cast<u64>(s) * a.groups];
+            if (FORWARD) {
+                const double count = static_cast<double>(part_rows(a, s)) * a.per_group, d = v.x - base;
+                first += count * d;
+                second += v.y + count * d * d;
+            } else {
+                first += v.x;
+                second += v.y;
+            }
+        }
+    sums[0][t] = first;
+    sums[1][t] = second;
+    for (unsigned int half = lanes / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (t < half * a.tile_groups) {
+            sums[0][t] += sums[0][t + half * a.tile_groups];
+            sums[1][t] += sums[1][t + half * a.tile_groups];
+        }
     }
-    m2 = lanes_sum_f64(m2);
-    if (lane == 0) {
-        a.stats[which * 2] = static_cast<float>(mean);
-        a.stats[which * 2 + 1] = static_cast<float>(1.0 / sqrt(m2 / total + static_cast<double>(a.eps)));
+    if (t < a.tile_groups) {  // (its own sums)
+        first = sums[0][t] * a.total_inverse;
+        second = sums[1][t] * a.total_inverse;
+        if (FORWARD) of(t, static_cast<float>(base + first), 1.0f / sqrtf(static_cast<float>(not_negative(second - first * first)) + a.eps));
+        else of(t, static_cast<float>(first), static_cast<float>(second));
+    }
+    __syncthreads();
+}
+
+template <class T, int V, int ACT, bool STREAM>
+__global__ void __launch_bounds__(kBlock) custos_group_norm_values(const GroupNormArgs a) {
+    const Stream<V> w(a, a.values, a.blocks - 1 - blockIdx.x);  // (backwards: what the first pass read last is in the caches)
+    __shared__ float2 stats[kMaxStreamGroups];
+    float2* written = reinterpret_cast<float2*>(a.stats) + static_cast<u64>(w.n) * a.groups + w.tile * a.tile_groups;
+    const bool writes = w.part == w.n * a.values.count;  // (one of the sample's workgroups writes the statistics down)
+    join_parts<true>(a, w.n, w.tile, [&](unsigned int g, float mean, float rstd) {
+        stats[g] = make_float2(mean, rstd);
+        if (writes) written[g] = stats[g];
+    });
+    if (w.rows == 0) return;
+    for (unsigned int col = w.col0; col < w.vecs; col += kBlock) {
+        const Column c = column_of<V>(a, col);
+        float scale[V], shift[V];
+        params<T, V>(a.gamma, a.param_f32, w.c0 + c.first, 1.0f, scale);
+        params<T, V>(a.beta, a.param_f32, w.c0 + c.first, 0.0f, shift);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const unsigned int g = a.tile_groups == 1 ? 0 : group_of(c.first + j, a.per_group_magic);
+            const float2 mean_rstd = stats[g];
+            scale[j] *= mean_rstd.y;
+            shift[j] = __builtin_fmaf(-mean_rstd.x, scale[j], shift[j]);
+        }
+        T* out = static_cast<T*>(a.out) + w.c0 + c.first;
+        {
+            auto value = [&](const Source<T, V, false>& x) {
+                Pack<T, V> y;
+#pragma unroll
+                for (int j = 0; j < V; j++)
+                    y.v[j] = from_f32<T>(act<ACT>(__builtin_fmaf(x.value(j), scale[j], shift[j])));
+                return y;
+            };
+            constexpr int kAhead = 4;
+            u64 i = 0;
+            for (; i + kAhead <= w.rows; i += kAhead) {
+                Source<T, V, false> x[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) x[u].template load<STREAM>(a, w.first + (i + u) * w.stride, w.c0 + c.first);
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) store_pack<STREAM, T, V>(out + (w.first + (i + u) * w.stride) * a.out_pitch, value(x[u]));
+            }
+            for (; i < w.rows; i++) {
+                Source<T, V, false> x;
+                x.template load<STREAM>(a, w.first + i * w.stride, w.c0 + c.first);
+                store_pack<STREAM, T, V>(out + (w.first + i * w.stride) * a.out_pitch, value(x));
+            }
+        }
     }
 }
+
+// ---- backward ----
 
 // What a thread needs of its column's channels.
 template <class T, int V>
@@ -438,79 +599,54 @@ struct ChannelParams {
     float mean[V], rstd[V], gamma[V], beta[V];
     __device__ __forceinline__ void load(const GroupNormArgs& a, unsigned int n, unsigned int tile, const Column& c) {
         const unsigned int c0 = tile * a.tile_groups * a.per_group;
-        const float* stats = a.stats + (static_cast<u64>(n) * a.groups + tile * a.tile_groups) * 2;
+        const float2* stats = reinterpret_cast<const float2*>(a.stats) + static_cast<u64>(n) * a.groups + tile * a.tile_groups;
+        params<T, V>(a.gamma, a.param_f32, c0 + c.first, 1.0f, gamma);
+        params<T, V>(a.beta, a.param_f32, c0 + c.first, 0.0f, beta);
+        if (a.whole_groups) {  // (the vector's channels are one group's)
+            const float2 s = stats[a.tile_groups == 1 ? 0 : group_of(c.first, a.per_group_magic)];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const unsigned int g = a.tile_groups == 1 ? 0 : group_of(c.first + j, a.per_group_magic);
-            mean[j] = stats[g * 2];
-            rstd[j] = stats[g * 2 + 1];
-            gamma[j] = param<T>(a.gamma, a.param_f32, c0 + c.first + j, 1.0f);
-            beta[j] = param<T>(a.beta, a.param_f32, c0 + c.first + j, 0.0f);
+            for (int j = 0; j < V; j++) mean[j] = s.x, rstd[j] = s.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float2 s = stats[group_of(c.first + j, a.per_group_magic)];
+                mean[j] = s.x;
+                rstd[j] = s.y;
+            }
         }
     }
 };
 
-template <class T, int V>
-__global__ void __launch_bounds__(kBlock) custos_group_norm_values(const GroupNormArgs a) {
-    const unsigned int t = threadIdx.x;
-    const unsigned int part = blockIdx.x / a.tiles, tile = blockIdx.x - part * a.tiles;
-    const unsigned int n = part / a.splits, split = part - n * a.splits;
-    const u64 p0 = split * a.rows, p1 = min(p0 + a.rows, a.positions);
-    const unsigned int vecs = (a.tile_groups * a.per_group + V - 1) / V;
-    const bool one_column = vecs <= kBlock;
-    const unsigned int step = one_column ? kBlock / vecs : 1;
-    const unsigned int r0 = one_column ? t / vecs : 0;
-    if (r0 >= step || p0 + r0 >= p1) return;
-    const u64 rows = (p1 - p0 - r0 + step - 1) / step;
-    const u64 first = static_cast<u64>(n) * a.positions + p0 + r0;
-    const unsigned int c0 = tile * a.tile_groups * a.per_group;
-    for (unsigned int col = one_column ? t - r0 * vecs : t; col < vecs; col += kBlock) {
-        const Column c = column_of<V>(a, col);
-        ChannelParams<T, V> k;
-        k.load(a, n, tile, c);
-        T* out = static_cast<T*>(a.out) + c0 + c.first;
-        with_activation(a.activation, [&](auto which) {
-            constexpr int kAct = decltype(which)::value;
-            auto value = [&](const Source<T, V, false>& x) {
-                Pack<T, V> y;
-#pragma unroll
-                for (int j = 0; j < V; j++)
-                    y.v[j] = from_f32<T>(act<kAct>((x.value(j) - k.mean[j]) * k.rstd[j] * k.gamma[j] + k.beta[j]));
-                return y;
-            };
-            constexpr int kAhead = 4;
-            u64 i = 0;
-            for (; i + kAhead <= rows; i += kAhead) {
-                Source<T, V, false> x[kAhead];
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) x[u].load(a, first + (i + u) * step, c0 + c.first);
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) store_valid<T, V>(out + (first + (i + u) * step) * a.out_pitch, value(x[u]), c.dup);
-            }
-            for (; i < rows; i++) {
-                Source<T, V, false> x;
-                x.load(a, first + i * step, c0 + c.first);
-                store_valid<T, V>(out + (first + i * step) * a.out_pitch, value(x), c.dup);
-            }
-        });
-    }
-}
-
-// ---- backward ----
-//
-// Work area: for every sample and part [2][channels] sums of dz and of dz * h (`partial`); joined over the
-// parts, [samples][2][channels] (in the place of part 0); and [samples][groups] pairs of the two means over a group (`sums`).
-
-// dz and h of one element.
-template <int ACT>
-__device__ __forceinline__ float dz_of(float x, float out_grad, float mean, float rstd, float gamma, float beta, float* h) {
-    *h = (x - mean) * rstd;
-    const float z = *h * gamma + beta;
+// dz and h of element j of a column.
+template <int ACT, class T, int V>
+__device__ __forceinline__ float dz_of(const ChannelParams<T, V>& k, int j, float x, float out_grad, float* h) {
+    *h = (x - k.mean[j]) * k.rstd[j];
+    const float z = *h * k.gamma[j] + k.beta[j];
     return out_grad * act_grad<ACT>(z);
 }
 
+// x_grad = rstd * (dz * gamma - mean_dh - h * mean_dhh), the rstd multiplied in beforehand.
 template <class T, int V>
-__device__ __forceinline__ void store_grad(const GroupNormArgs& a, T* p, float (&g)[V], int dup) {
+struct GradientOf {
+    float on_dz[V], on_h[V], constant[V];
+    template <class F>
+    __device__ __forceinline__ GradientOf(const ChannelParams<T, V>& k, F means_of) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            float dh, dhh;
+            means_of(j, &dh, &dhh);
+            on_dz[j] = k.rstd[j] * k.gamma[j];
+            on_h[j] = -k.rstd[j] * dhh;
+            constant[j] = -k.rstd[j] * dh;
+        }
+    }
+    __device__ __forceinline__ float of(int j, float dz, float h) const {
+        return __builtin_fmaf(dz, on_dz[j], __builtin_fmaf(h, on_h[j], constant[j]));
+    }
+};
+
+template <bool STREAM, class T, int V>
+__device__ __forceinline__ void store_grad(const GroupNormArgs& a, T* p, float (&g)[V]) {
     Pack<T, V> y;
     if (a.accumulate) {
         const Pack<T, V> was = load_pack<false, T, V>(p);
@@ -519,37 +655,116 @@ __device__ __forceinline__ void store_grad(const GroupNormArgs& a, T* p, float (
     }
 #pragma unroll
     for (int j = 0; j < V; j++) y.v[j] = from_f32<T>(g[j]);
-    store_valid<T, V>(p, y, dup);
+    store_pack<STREAM, T, V>(p, y);
+}
+
+// From a thread's sums s1 (dz) and s2 (dz * h) of its column: those of the channels over the rows of the workgroup,
+// to `channel`, and from there, times gamma, those of the groups, to sums_of.
+template <int V, int THREADS>
+__device__ __forceinline__ void channel_and_group_sums(const GroupNormArgs& a, const Column& c, unsigned int r0, unsigned int step,
+                                                       const float (&s1)[V], const float (&s2)[V], const float (&gamma_of)[V], float2* table, float* gammas,
+                                                       float* channel, float2* sums_of) {
+    const unsigned int t = threadIdx.x;
+    if (r0 == 0) {
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            if (j >= c.dup) gammas[c.first + j] = gamma_of[j];
+    }
+    if (r0 < step) {
+        float2* row = table + r0 * c.width + c.first;
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            if (j >= c.dup) row[j] = make_float2(s1[j], s2[j]);
+    }
+    __syncthreads();
+    // (a power of two of neighbouring lanes for each channel, then for each group)
+    unsigned int lanes = 1;
+    while (lanes < 64 && lanes * 2 * c.width <= static_cast<unsigned int>(THREADS) && lanes < step) lanes *= 2;
+    for (unsigned int base = 0; base < c.width; base += THREADS / lanes) {
+        const unsigned int ch = base + t / lanes;
+        float x = 0.0f, y = 0.0f;
+        if (ch < c.width)
+            for (unsigned int r = t % lanes; r < step; r += lanes) {
+                const float2 v = table[r * c.width + ch];
+                x += v.x;
+                y += v.y;
+            }
+        for (unsigned int half = lanes / 2; half > 0; half /= 2) x += __shfl_xor(x, half, 64), y += __shfl_xor(y, half, 64);
+        if (ch < c.width && t % lanes == 0) {
+            channel[ch] = x;
+            channel[a.channels + ch] = y;
+            const float gamma = gammas[ch];
+            table[ch] = make_float2(x * gamma, y * gamma);  // (only these lanes read column ch, and they have)
+        }
+    }
+    __syncthreads();
+    lanes = 1;
+    while (lanes < 64 && lanes * 2 * a.tile_groups <= static_cast<unsigned int>(THREADS) && lanes < a.per_group) lanes *= 2;
+    for (unsigned int base = 0; base < a.tile_groups; base += THREADS / lanes) {
+        const unsigned int g = base + t / lanes;
+        float x = 0.0f, y = 0.0f;
+        if (g < a.tile_groups)
+            for (unsigned int i = t % lanes; i < a.per_group; i += lanes) {
+                const float2 v = table[g * a.per_group + i];
+                x += v.x;
+                y += v.y;
+            }
+        for (unsigned int half = lanes / 2; half > 0; half /= 2) x += __shfl_xor(x, half, 64), y += __shfl_xor(y, half, 64);
+        if (g < a.tile_groups && t % lanes == 0) sums_of[g] = make_float2(x, y);
+    }
+    __syncthreads();
+}
+
+// gamma_grad and beta_grad of 16 channels, by one workgroup: the sums of all parts of all samples, in a fixed order.
+constexpr int kParamChannels = 16;
+__device__ __forceinline__ void param_grads(const GroupNormArgs& a, unsigned int block, float* sums) {
+    const unsigned int t = threadIdx.x, which = t / kParamChannels % 2, lane = t / (2 * kParamChannels);
+    constexpr unsigned int kLanes = kBlock / (2 * kParamChannels);
+    const unsigned int ch = block * kParamChannels + t % kParamChannels;
+    float s = 0.0f;
+    if (ch < a.channels)
+#pragma unroll 4
+        for (unsigned int row = lane; row < a.samples * a.parts.count; row += kLanes)
+            s += a.channel_parts[(static_cast<u64>(row) * 2 + which) * a.channels + ch];
+    sums[t] = s;
+    __syncthreads();
+    if (lane > 0 || ch >= a.channels) return;
+    for (unsigned int l = 1; l < kLanes; l++) s += sums[l * 2 * kParamChannels + t];
+    float* out = which ? a.gamma_grad : a.beta_grad;
+    if (out) out[ch] = a.accumulate ? out[ch] + s : s;
+}
+
+__global__ void __launch_bounds__(kBlock) custos_group_norm_param_grads(const GroupNormArgs a) {
+    __shared__ float sums[kBlock];
+    param_grads(a, blockIdx.x, sums);
 }
 
 // A tile in registers: x and out_grad read once.
-template <class T, int V, int HELD, int THREADS, bool SAVED>
+template <class T, int V, int HELD, int THREADS, bool SAVED, int ACT>
 __global__ void __launch_bounds__(THREADS) custos_group_norm_grad_tile(const GroupNormArgs a) {
-    __shared__ float table[THREADS * V];
-    __shared__ float wave_sums[THREADS / 64];
-    __shared__ float sum_dh[kMaxTileGroups], sum_dhh[kMaxTileGroups];
+    __shared__ float2 table[THREADS * V];
+    __shared__ float gammas[THREADS * V];
+    __shared__ float2 sums_of[kMaxTileGroups];
     const unsigned int t = threadIdx.x;
-    const unsigned int n = blockIdx.x / a.tiles, tile = blockIdx.x - n * a.tiles;
-    const unsigned int vecs = (a.tile_groups * a.per_group + V - 1) / V;
-    const unsigned int step = THREADS / vecs;
-    const unsigned int r0 = t / vecs;
+    const unsigned int index = by_xcd(blockIdx.x, gridDim.x), n = a.by_tiles.divide(index), tile = index - n * a.tiles;
+    const unsigned int vecs = a.vecs, step = a.step;
+    const unsigned int r0 = group_of(t, a.vecs_magic);
     const Column c = column_of<V>(a, t - r0 * vecs);
     const bool active = r0 < step;
     const unsigned int c0 = tile * a.tile_groups * a.per_group;
     const u64 row0 = static_cast<u64>(n) * a.positions;
     const T* out_grad = static_cast<const T*>(a.out_grad) + row0 * a.grad_pitch + c0 + c.first;
     Source<T, V, SAVED> held[HELD];
-    Pack<T, V> grad[HELD];
+    Bits<T, V> grad[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
         const u64 p = r0 + static_cast<u64>(i) * step;
         if (active && p < a.positions) {
             held[i].load(a, row0 + p, c0 + c.first);
-            grad[i] = load_pack<false, T, V>(out_grad + p * a.grad_pitch);
+            grad[i].load(out_grad + p * a.grad_pitch);
         } else {
             held[i].zero();
-#pragma unroll
-            for (int j = 0; j < V; j++) grad[i].v[j] = from_f32<T>(0.0f);
+            grad[i].zero();
         }
     }
     ChannelParams<T, V> k;
@@ -557,47 +772,32 @@ __global__ void __launch_bounds__(THREADS) custos_group_norm_grad_tile(const Gro
     float s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.0f;
-    with_activation(a.activation, [&](auto which) {
+    {
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
             if (r0 + static_cast<u64>(i) * step >= a.positions) break;
 #pragma unroll
             for (int j = 0; j < V; j++) {
                 float h;
-                const float dz = dz_of<decltype(which)::value>(held[i].value(j), to_f32(grad[i].v[j]), k.mean[j], k.rstd[j],
-                                                               k.gamma[j], k.beta[j], &h);
+                const float dz = dz_of<ACT>(k, j, held[i].value(j), to_f32(grad[i].pack().v[j]), &h);
                 s1[j] += dz;
                 s2[j] = __builtin_fmaf(dz, h, s2[j]);
             }
+            held[i].forget_values();
+            grad[i].forget_values();
         }
-    });
-    // over the rows of the workgroup: per channel, which is what the gradients of gamma and beta need, and
-    // from there per group
-    float* channel = a.partial + static_cast<u64>(n) * 2 * a.channels + c0;
-    for (int which = 0; which < 2; which++) {
-#pragma unroll
-        for (int j = 0; j < V; j++)
-            if (active && j >= c.dup) table[r0 * c.width + c.first + j] = which ? s2[j] : s1[j];
-        __syncthreads();
-        for (unsigned int ch = t; ch < c.width; ch += THREADS) {
-            float s = 0.0f;
-            for (unsigned int r = 0; r < step; r++) s += table[r * c.width + ch];
-            channel[static_cast<u64>(which) * a.channels + ch] = s;
-            table[ch] = s * param<T>(a.gamma, a.param_f32, c0 + ch, 1.0f);
-        }
-        group_sums<THREADS>(table, 1, c.width, a.tile_groups, a.per_group, a.per_group_magic, wave_sums, which ? sum_dhh : sum_dh);
     }
+    channel_and_group_sums<V, THREADS>(a, c, r0, step, s1, s2, k.gamma, table, gammas, a.channel_parts + static_cast<u64>(n) * 2 * a.channels + c0, sums_of);
     if (!a.out || !active) return;
     const float count = static_cast<float>(a.positions) * static_cast<float>(a.per_group);
-    float mean_dh[V], mean_dhh[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) {
+    const GradientOf<T, V> gradient(k, [&](int j, float* dh, float* dhh) {
         const unsigned int g = group_of(c.first + j, a.per_group_magic);
-        mean_dh[j] = sum_dh[g] / count;
-        mean_dhh[j] = sum_dhh[g] / count;
-    }
+        const float2 both = sums_of[g];
+        *dh = both.x / count;
+        *dhh = both.y / count;
+    });
     T* out = static_cast<T*>(a.out) + row0 * a.out_pitch + c0 + c.first;
-    with_activation(a.activation, [&](auto which) {
+    {
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
             const u64 p = r0 + static_cast<u64>(i) * step;
@@ -606,255 +806,183 @@ __global__ void __launch_bounds__(THREADS) custos_group_norm_grad_tile(const Gro
 #pragma unroll
             for (int j = 0; j < V; j++) {
                 float h;
-                const float dz = dz_of<decltype(which)::value>(held[i].value(j), to_f32(grad[i].v[j]), k.mean[j], k.rstd[j],
-                                                               k.gamma[j], k.beta[j], &h);
-                g[j] = k.rstd[j] * (dz * k.gamma[j] - mean_dh[j] - h * mean_dhh[j]);
+                const float dz = dz_of<ACT>(k, j, held[i].value(j), to_f32(grad[i].pack().v[j]), &h);
+                g[j] = gradient.of(j, dz, h);
             }
-            store_grad<T, V>(a, out + p * a.out_pitch, g, c.dup);
+            store_grad<false, T, V>(a, out + p * a.out_pitch, g);
         }
-    });
+    }
 }
 
-// Sums of dz and dz * h per channel over the rows of one part.
-template <class T, int V, bool SAVED>
+// Rows of x and out_grad, `kAhead` of them loaded before they are used.
+template <class T, int V, bool SAVED, bool STREAM, class F>
+__device__ __forceinline__ void for_rows(const GroupNormArgs& a, const Stream<V>& w, unsigned int channel, F f) {
+    const T* out_grad = static_cast<const T*>(a.out_grad) + channel;
+    constexpr int kAhead = 2;
+    u64 i = 0;
+    for (; i + kAhead <= w.rows; i += kAhead) {
+        Source<T, V, SAVED> x[kAhead];
+        Bits<T, V> g[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const u64 row = w.first + (i + u) * w.stride;
+            x[u].template load<STREAM>(a, row, channel);
+            g[u].template load<STREAM>(out_grad + row * a.grad_pitch);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) f(w.first + (i + u) * w.stride, x[u], g[u].pack());
+    }
+    for (; i < w.rows; i++) {
+        const u64 row = w.first + i * w.stride;
+        Source<T, V, SAVED> x;
+        Bits<T, V> g;
+        x.template load<STREAM>(a, row, channel);
+        g.template load<STREAM>(out_grad + row * a.grad_pitch);
+        f(row, x, g.pack());
+    }
+}
+
+// Sums of dz and dz * h over the rows of one part: per channel, and times gamma per group.
+template <class T, int V, bool SAVED, int ACT>
 __global__ void __launch_bounds__(kBlock) custos_group_norm_grad_parts(const GroupNormArgs a) {
-    __shared__ float table[kBlock * V];
+    __shared__ float2 table[kBlock * V];
+    __shared__ float gammas[kBlock * V];
+    __shared__ float2 sums_of[kMaxStreamGroups];
+    __shared__ float wave_sums[kBlock / 64];
     const unsigned int t = threadIdx.x;
-    const unsigned int part = blockIdx.x / a.tiles, tile = blockIdx.x - part * a.tiles;
-    const unsigned int n = part / a.splits, split = part - n * a.splits;
-    const u64 p0 = split * a.rows, p1 = min(p0 + a.rows, a.positions);
-    const unsigned int vecs = (a.tile_groups * a.per_group + V - 1) / V;
-    const bool one_column = vecs <= kBlock;
-    const unsigned int step = one_column ? kBlock / vecs : 1;
-    const unsigned int r0 = one_column ? t / vecs : 0;
-    const u64 rows = r0 < step && p0 + r0 < p1 ? (p1 - p0 - r0 + step - 1) / step : 0;
-    const u64 first = static_cast<u64>(n) * a.positions + p0 + r0;
-    const unsigned int c0 = tile * a.tile_groups * a.per_group;
-    float* channel = a.partial + static_cast<u64>(part) * 2 * a.channels + c0;
-    float s1[V], s2[V];
-    Column c = column_of<V>(a, one_column ? t - r0 * vecs : t);
-    for (unsigned int col = one_column ? t - r0 * vecs : t; col < vecs && r0 < step; col += kBlock) {
+    const Stream<V> w(a, a.parts, blockIdx.x);
+    float* channel = a.channel_parts + static_cast<u64>(w.part) * 2 * a.channels + w.c0;
+    float* group = a.group_parts + (static_cast<u64>(w.part) * a.groups + w.tile * a.tile_groups) * 2;
+    float s1[V], s2[V], dh = 0.0f, dhh = 0.0f;
+    ChannelParams<T, V> k;
+#pragma unroll
+    for (int j = 0; j < V; j++) s1[j] = s2[j] = k.gamma[j] = 0.0f;
+    Column c = column_of<V>(a, w.col0);
+    for (unsigned int col = w.col0; col < w.vecs && w.active(); col += kBlock) {
         c = column_of<V>(a, col);
 #pragma unroll
         for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.0f;
-        ChannelParams<T, V> k;
-        k.load(a, n, tile, c);
-        const T* out_grad = static_cast<const T*>(a.out_grad) + c0 + c.first;
-        with_activation(a.activation, [&](auto which) {
-            auto add = [&](const Source<T, V, SAVED>& x, const Pack<T, V>& g) {
+        k.load(a, w.n, w.tile, c);
+        {
+            for_rows<T, V, SAVED, false>(a, w, w.c0 + c.first, [&](u64, const Source<T, V, SAVED>& x, const Pack<T, V>& g) {
 #pragma unroll
                 for (int j = 0; j < V; j++) {
                     float h;
-                    const float dz = dz_of<decltype(which)::value>(x.value(j), to_f32(g.v[j]), k.mean[j], k.rstd[j], k.gamma[j],
-                                                                   k.beta[j], &h);
+                    const float dz = dz_of<ACT>(k, j, x.value(j), to_f32(g.v[j]), &h);
                     s1[j] += dz;
                     s2[j] = __builtin_fmaf(dz, h, s2[j]);
                 }
-            };
-            constexpr int kAhead = 2;
-            u64 i = 0;
-            for (; i + kAhead <= rows; i += kAhead) {
-                Source<T, V, SAVED> x[kAhead];
-                Pack<T, V> g[kAhead];
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) {
-                    const u64 row = first + (i + u) * step;
-                    x[u].load(a, row, c0 + c.first);
-                    g[u] = load_pack<false, T, V>(out_grad + row * a.grad_pitch);
-                }
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) add(x[u], g[u]);
-            }
-            for (; i < rows; i++) {
-                Source<T, V, SAVED> x;
-                x.load(a, first + i * step, c0 + c.first);
-                add(x, load_pack<false, T, V>(out_grad + (first + i * step) * a.grad_pitch));
-            }
-        });
-        if (!one_column) {
+            });
+        }
+        if (!w.one_column) {
 #pragma unroll
             for (int j = 0; j < V; j++)
-                if (j >= c.dup) channel[c.first + j] = s1[j], channel[a.channels + c.first + j] = s2[j];
+                if (j >= c.dup) {
+                    channel[c.first + j] = s1[j], channel[a.channels + c.first + j] = s2[j];
+                    dh = __builtin_fmaf(s1[j], k.gamma[j], dh);
+                    dhh = __builtin_fmaf(s2[j], k.gamma[j], dhh);
+                }
         }
     }
-    if (!one_column) return;
-    const bool active = r0 < step;
-    for (int which = 0; which < 2; which++) {
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < V; j++)
-            if (active && j >= c.dup) table[r0 * c.width + c.first + j] = which ? s2[j] : s1[j];
-        __syncthreads();
-        for (unsigned int ch = t; ch < c.width; ch += kBlock) {
-            float s = 0.0f;
-            for (unsigned int r = 0; r < step; r++) s += table[r * c.width + ch];
-            channel[static_cast<u64>(which) * a.channels + ch] = s;
-        }
+    if (!w.one_column) {
+        dh = block_sum<kBlock>(dh, wave_sums);
+        dhh = block_sum<kBlock>(dhh, wave_sums);
+        if (t == 0) group[0] = dh, group[1] = dhh;
+        return;
     }
+    channel_and_group_sums<V, kBlock>(a, c, w.r0, w.step, s1, s2, k.gamma, table, gammas, channel, sums_of);
+    for (unsigned int g = t; g < a.tile_groups; g += kBlock) reinterpret_cast<float2*>(group)[g] = sums_of[g];
 }
 
-// The parts of a sample joined, one workgroup for every sample and group: per channel (over the part 0 sums),
-// and the two means over the group.
-template <class T>
-__global__ void __launch_bounds__(kBlock) custos_group_norm_grad_sums(const GroupNormArgs a) {
-    __shared__ float table[2 * kBlock];
-    __shared__ float wave_sums[kBlock / 64];
-    const unsigned int t = threadIdx.x;
-    const unsigned int n = blockIdx.x / a.groups, g = blockIdx.x - n * a.groups;
-    const unsigned int c0 = g * a.per_group;
-    float* part = a.partial + static_cast<u64>(n) * a.splits * 2 * a.channels + c0;
-    float dh = 0.0f, dhh = 0.0f;
-    // (threads over the channels, and over the parts where there are fewer channels than threads)
-    const unsigned int cols = min(a.per_group, static_cast<unsigned int>(kBlock)), lanes = kBlock / cols;
-    const unsigned int r = t / cols;
-    for (unsigned int base = 0; base < a.per_group; base += cols) {
-        const unsigned int ch = base + (t - r * cols);
-        const bool active = r < lanes && ch < a.per_group;
-        float s1 = 0.0f, s2 = 0.0f;
-        if (active)
-            for (unsigned int s = r; s < a.splits; s += lanes) {
-                s1 += part[static_cast<u64>(s) * 2 * a.channels + ch];
-                s2 += part[(static_cast<u64>(s) * 2 + 1) * a.channels + ch];
-            }
-        __syncthreads();
-        table[t] = s1;
-        table[kBlock + t] = s2;
-        __syncthreads();
-        if (!active || r != 0) continue;
-        for (unsigned int l = 1; l < lanes; l++) {
-            s1 += table[l * cols + t];
-            s2 += table[kBlock + l * cols + t];
-        }
-        part[ch] = s1;
-        part[a.channels + ch] = s2;
-        const float gamma = param<T>(a.gamma, a.param_f32, c0 + ch, 1.0f);
-        dh += s1 * gamma;
-        dhh += s2 * gamma;
-    }
-    dh = block_sum<kBlock>(dh, wave_sums);
-    dhh = block_sum<kBlock>(dhh, wave_sums);
-    if (t == 0) {
-        const float count = static_cast<float>(a.positions) * static_cast<float>(a.per_group);
-        a.sums[(static_cast<u64>(n) * a.groups + g) * 2] = dh / count;
-        a.sums[(static_cast<u64>(n) * a.groups + g) * 2 + 1] = dhh / count;
-    }
-}
-
-template <class T, int V, bool SAVED>
+// x_grad, and by the workgroups behind the first `blocks` gamma_grad and beta_grad.
+template <class T, int V, bool SAVED, int ACT, bool STREAM>
 __global__ void __launch_bounds__(kBlock) custos_group_norm_grad_values(const GroupNormArgs a) {
-    const unsigned int t = threadIdx.x;
-    const unsigned int part = blockIdx.x / a.tiles, tile = blockIdx.x - part * a.tiles;
-    const unsigned int n = part / a.splits, split = part - n * a.splits;
-    const u64 p0 = split * a.rows, p1 = min(p0 + a.rows, a.positions);
-    const unsigned int vecs = (a.tile_groups * a.per_group + V - 1) / V;
-    const bool one_column = vecs <= kBlock;
-    const unsigned int step = one_column ? kBlock / vecs : 1;
-    const unsigned int r0 = one_column ? t / vecs : 0;
-    if (r0 >= step || p0 + r0 >= p1) return;
-    const u64 rows = (p1 - p0 - r0 + step - 1) / step;
-    const u64 first = static_cast<u64>(n) * a.positions + p0 + r0;
-    const unsigned int c0 = tile * a.tile_groups * a.per_group;
-    const float* sums = a.sums + (static_cast<u64>(n) * a.groups + tile * a.tile_groups) * 2;
-    for (unsigned int col = one_column ? t - r0 * vecs : t; col < vecs; col += kBlock) {
+    __shared__ float sums[kBlock];
+    if (blockIdx.x >= a.blocks) {
+        param_grads(a, blockIdx.x - a.blocks, sums);
+        return;
+    }
+    const Stream<V> w(a, a.values, a.blocks - 1 - blockIdx.x);  // (backwards: what the first pass read last is in the caches)
+    __shared__ float2 means[kMaxStreamGroups];
+    join_parts<false>(a, w.n, w.tile, [&](unsigned int g, float dh, float dhh) { means[g] = make_float2(dh, dhh); });
+    if (w.rows == 0) return;
+    for (unsigned int col = w.col0; col < w.vecs; col += kBlock) {
         const Column c = column_of<V>(a, col);
         ChannelParams<T, V> k;
-        k.load(a, n, tile, c);
-        float mean_dh[V], mean_dhh[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) {
+        k.load(a, w.n, w.tile, c);
+        const GradientOf<T, V> gradient(k, [&](int j, float* dh, float* dhh) {
             const unsigned int g = a.tile_groups == 1 ? 0 : group_of(c.first + j, a.per_group_magic);
-            mean_dh[j] = sums[g * 2];
-            mean_dhh[j] = sums[g * 2 + 1];
-        }
-        const T* out_grad = static_cast<const T*>(a.out_grad) + c0 + c.first;
-        T* out = static_cast<T*>(a.out) + c0 + c.first;
-        with_activation(a.activation, [&](auto which) {
-            auto put = [&](u64 row, const Source<T, V, SAVED>& x, const Pack<T, V>& og) {
+            const float2 both = means[g];
+            *dh = both.x;
+            *dhh = both.y;
+        });
+        T* out = static_cast<T*>(a.out) + w.c0 + c.first;
+        {
+            for_rows<T, V, SAVED, STREAM>(a, w, w.c0 + c.first, [&](u64 row, const Source<T, V, SAVED>& x, const Pack<T, V>& og) {
                 float g[V];
 #pragma unroll
                 for (int j = 0; j < V; j++) {
                     float h;
-                    const float dz = dz_of<decltype(which)::value>(x.value(j), to_f32(og.v[j]), k.mean[j], k.rstd[j], k.gamma[j],
-                                                                   k.beta[j], &h);
-                    g[j] = k.rstd[j] * (dz * k.gamma[j] - mean_dh[j] - h * mean_dhh[j]);
+                    const float dz = dz_of<ACT>(k, j, x.value(j), to_f32(og.v[j]), &h);
+                    g[j] = gradient.of(j, dz, h);
                 }
-                store_grad<T, V>(a, out + row * a.out_pitch, g, c.dup);
-            };
-            constexpr int kAhead = 2;
-            u64 i = 0;
-            for (; i + kAhead <= rows; i += kAhead) {
-                Source<T, V, SAVED> x[kAhead];
-                Pack<T, V> g[kAhead];
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) {
-                    const u64 row = first + (i + u) * step;
-                    x[u].load(a, row, c0 + c.first);
-                    g[u] = load_pack<false, T, V>(out_grad + row * a.grad_pitch);
-                }
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) put(first + (i + u) * step, x[u], g[u]);
-            }
-            for (; i < rows; i++) {
-                const u64 row = first + i * step;
-                Source<T, V, SAVED> x;
-                x.load(a, row, c0 + c.first);
-                put(row, x, load_pack<false, T, V>(out_grad + row * a.grad_pitch));
-            }
-        });
+                store_grad<STREAM, T, V>(a, out + row * a.out_pitch, g);
+            });
+        }
     }
-}
-
-// gamma_grad and beta_grad: the channel sums of the samples, added in their order.
-__global__ void __launch_bounds__(kBlock) custos_group_norm_param_grads(const float* sums, u64 sample_stride, unsigned int samples,
-                                                                        unsigned int channels, float* gamma_grad, float* beta_grad,
-                                                                        int accumulate) {
-    const unsigned int ch = blockIdx.x * kBlock + threadIdx.x;
-    if (ch >= channels) return;
-    float s1 = 0.0f, s2 = 0.0f;
-    for (unsigned int n = 0; n < samples; n++) {
-        s1 += sums[n * sample_stride + ch];
-        s2 += sums[n * sample_stride + channels + ch];
-    }
-    if (beta_grad) beta_grad[ch] = accumulate ? beta_grad[ch] + s1 : s1;
-    if (gamma_grad) gamma_grad[ch] = accumulate ? gamma_grad[ch] + s2 : s2;
 }
 
 // ---- host ----
+
+// What the plans below go by, in microseconds measured on MI355X (kernels alone):
+// - Rows of a tile in registers are at least 32 bytes: twice the workgroups of 64-byte rows, 8x1024x640 bf16 in
+//   12.8 against 14.6 (41 with 128 bytes); the tiles that share a cache line run on one XCD.
+// - Rows of a tile that is streamed are at least 128 bytes: the second pass of the gradient over 4x4096x320 bf16
+//   takes 10.9, with 256 bytes 12.2, with 64 bytes 15.2; the first pass 11.8, 11.4, 13.7.  Where the data does not
+//   stay in the caches, 256 bytes: gradient over 8x16384x512 bf16 from codes 49 + 57, with 128 bytes 50 + 79, with
+//   512 bytes 48 + 60.
+// - A tile of more than 16384 values is only held if there are at least 128 of them: 33 tiles of 58830 f32 values
+//   with GELU take 28 on 33 of 256 CUs, two streaming passes over the same data 16.
+// - Beyond 64 MiB moved the second pass loads and stores past the caches: its results would only push out what the
+//   first pass read and leave dirty lines to be written back during the next pass.  16x16384x512 f16: first pass
+//   55 and second 88 that way, 85 and 102 through the caches.
+constexpr unsigned int kTileRow = 32, kStreamRow = 128;
+constexpr u64 kTileAlone = 16384, kTilesTogether = 128, kStreamBeyond = 64ull << 20;
 
 struct Plan {
     int vec = 1;                // channels per thread
     bool in_registers = false;
     int threads = kBlock;
     int held = 0;
+    bool stream = false;  // the second pass loads and stores past the caches
     GroupNormArgs a{};
 };
 
+Divisor divisor(unsigned int by) { return {by, by == 1 ? 0u : static_cast<unsigned int>(0x100000000ull / by)}; }
+
 unsigned int magic_of(unsigned int d) { return d == 1 ? 0u : static_cast<unsigned int>((0x100000000ull + d - 1) / d); }
 
-// The smallest divisor of `groups` whose tile is at least `channels` wide (or all groups); 0: more groups than
-// the kernels that hold a tile take.
-unsigned int tile_at_least(unsigned int groups, unsigned int per_group, unsigned int channels) {
-    for (unsigned int k = 1; k <= std::min<unsigned int>(groups, kMaxTileGroups); k++)
-        if (groups % k == 0 && (static_cast<u64>(k) * per_group >= channels || k == groups)) return k;
-    return 0;
+// The smallest divisor of `groups` whose tile is at least `channels` wide (or all groups); if it is above `most`,
+// the largest one below.
+unsigned int tile_at_least(unsigned int groups, unsigned int per_group, unsigned int channels, unsigned int most) {
+    unsigned int best = 1;
+    for (unsigned int k = 1; k <= std::min(groups, most); k++)
+        if (groups % k == 0) {
+            best = k;
+            if (static_cast<u64>(k) * per_group >= channels) break;
+        }
+    return best;
 }
-// The largest divisor of `groups` whose rows take at most kBlock vectors (or one group).
-unsigned int tile_at_most(unsigned int groups, unsigned int per_group, unsigned int vec) {
-    const u64 most = std::min<u64>(groups, static_cast<u64>(kBlock) * vec / per_group);
-    for (unsigned int k = static_cast<unsigned int>(most); k > 1; k--)
-        if (groups % k == 0) return k;
-    return 1;
-}
-
 // (threads, vectors held) of the kernels that hold a tile in registers, smallest first.
 struct Held {
     int threads, held;
 };
-constexpr Held kForwardHeld[] = {{256, 4}, {256, 16}, {1024, 16}};
+constexpr Held kForwardHeld[] = {{256, 4}, {256, 8}, {1024, 4}, {1024, 8}, {1024, 16}};
 constexpr Held kBackwardHeld[] = {{256, 4}, {1024, 4}};
 
+// `accumulates`: the results are added to what is there, so no channel may be stored by two threads.
 template <size_t N>
-void make_plan(const custos_hip_group_norm_desc& d, size_t elem, const Held (&choices)[N], Plan* plan) {
+void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool accumulates, const Held (&choices)[N], Plan* plan) {
     GroupNormArgs& a = plan->a;
     a.positions = d.positions;
     a.samples = static_cast<unsigned int>(d.samples);
@@ -862,43 +990,78 @@ void make_plan(const custos_hip_group_norm_desc& d, size_t elem, const Held (&ch
     a.groups = static_cast<unsigned int>(d.groups);
     a.per_group = a.channels / a.groups;
     a.per_group_magic = magic_of(a.per_group);
-    a.activation = d.activation;
     a.eps = static_cast<float>(d.eps);
     const unsigned int full = static_cast<unsigned int>(16 / elem);
+    auto finish = [&](u64 parts, u64 values) {
+        a.part_step = a.step;
+        const u64 rounds = (a.positions + a.step - 1) / a.step;
+        for (auto [of, count] : {std::pair<Splits*, u64>{&a.parts, parts}, std::pair<Splits*, u64>{&a.values, values}}) {
+            of->count = static_cast<unsigned int>(count);
+            of->rounds = rounds / count;
+            of->longer = static_cast<unsigned int>(rounds % count);
+            of->by_count = divisor(of->count);
+        }
+        a.last_part = static_cast<unsigned int>((rounds - 1) % parts);
+        a.missing_rows = static_cast<unsigned int>(rounds * a.step - a.positions);
+        a.by_tiles = divisor(a.tiles);
+        a.vecs_magic = magic_of(a.vecs);
+        a.waves_per_group = std::max(1u, static_cast<unsigned int>(plan->threads) / 64 / a.tile_groups);
+        a.waves_magic = magic_of(a.waves_per_group);
+        a.whole_groups = a.tile_groups == 1 || a.per_group % static_cast<unsigned int>(plan->vec) == 0;
+        a.total_inverse = 1.0 / (static_cast<double>(a.positions) * a.per_group);
+    };
     // in registers, if a tile of whole groups of at least 64 bytes a row fits
     {
-        const unsigned int k = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>(64 / elem));
+        const unsigned int k = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>(kTileRow / elem), kMaxTileGroups);
         const u64 width = static_cast<u64>(k) * a.per_group;
-        const unsigned int vec = width >= full ? full : 1;
+        const unsigned int vec = width < full || (accumulates && width % full != 0) ? 1 : full;
         const u64 vecs = (width + vec - 1) / vec;
         for (const Held& h : choices) {
-            if (k == 0 || vecs > static_cast<u64>(h.threads)) continue;
+            if (vecs > static_cast<u64>(h.threads)) continue;
             const u64 step = static_cast<u64>(h.threads) / vecs;
             if ((a.positions + step - 1) / step > static_cast<u64>(h.held)) continue;
+            if (a.positions * width > kTileAlone && static_cast<u64>(a.samples) * (a.groups / k) < kTilesTogether) continue;
             plan->in_registers = true;
             plan->vec = static_cast<int>(vec);
             plan->threads = h.threads;
             plan->held = h.held;
             a.tile_groups = k;
             a.tiles = a.groups / k;
-            a.splits = 1;
-            a.rows = a.positions;
+            a.vecs = static_cast<unsigned int>(vecs);
+            a.step = static_cast<unsigned int>(step);
+            finish(1, 1);
             return;
         }
     }
-    plan->vec = static_cast<int>(a.channels >= full ? full : 1);
-    a.tile_groups = tile_at_most(a.groups, a.per_group, static_cast<unsigned int>(plan->vec));
-    if (static_cast<u64>(a.tile_groups) * a.per_group < static_cast<u64>(plan->vec)) plan->vec = 1;
+    a.tile_groups = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>((moved > kStreamBeyond ? 2 * kStreamRow : kStreamRow) / elem), kMaxStreamGroups);
+    const u64 width = static_cast<u64>(a.tile_groups) * a.per_group;
+    plan->vec = static_cast<int>(width < full ? 1 : full);
     a.tiles = a.groups / a.tile_groups;
-    const u64 vecs = (static_cast<u64>(a.tile_groups) * a.per_group + plan->vec - 1) / plan->vec;
-    const u64 step = std::max<u64>(1, kBlock / vecs);
-    // parts: enough workgroups to fill the chip several times, each with a few rounds of rows
-    const u64 wanted = std::max<u64>(1, 2048 / (static_cast<u64>(a.samples) * a.tiles));
-    const u64 rounds = (a.positions + step - 1) / step;
-    u64 splits = std::min<u64>(wanted, std::max<u64>(1, rounds / 8));
-    a.rows = (rounds + splits - 1) / splits * step;
-    splits = (a.positions + a.rows - 1) / a.rows;
-    a.splits = static_cast<unsigned int>(splits);
+    const u64 vecs = (width + plan->vec - 1) / plan->vec;
+    a.vecs = static_cast<unsigned int>(vecs);
+    a.step = static_cast<unsigned int>(std::max<u64>(1, kBlock / vecs));
+    const u64 rounds = (a.positions + a.step - 1) / a.step, tiles = static_cast<u64>(a.samples) * a.tiles;
+    plan->stream = moved > kStreamBeyond;
+    // what the chip holds at once, each with a few rounds of rows, and no more parts than are joined in passing
+    finish(std::min<u64>({std::max<u64>(1, 1024 / tiles), std::max<u64>(1, rounds / 4), std::max<u64>(1, 4096 / a.tile_groups)}),
+           std::min<u64>(std::max<u64>(1, 2048 / tiles), std::max<u64>(1, rounds / 4)));
+}
+
+// The second pass of a streaming plan whose rows are no whole vectors and whose results are added to, or take the place
+// of, what it reads: channel by channel, so that none is stored, or read after it was stored, by another thread.
+void narrow_values(Plan* plan) {
+    GroupNormArgs& a = plan->a;
+    if (plan->vec == 1 || a.tile_groups * a.per_group % static_cast<unsigned int>(plan->vec) == 0) return;
+    plan->vec = 1;
+    a.vecs = a.tile_groups * a.per_group;
+    a.vecs_magic = magic_of(a.vecs);
+    a.step = std::max(1u, static_cast<unsigned int>(kBlock) / a.vecs);
+    a.whole_groups = 1;
+    const u64 rounds = (a.positions + a.step - 1) / a.step;
+    a.values.count = static_cast<unsigned int>(std::min<u64>(a.values.count, std::max<u64>(1, rounds / 4)));
+    a.values.rounds = rounds / a.values.count;
+    a.values.longer = static_cast<unsigned int>(rounds % a.values.count);
+    a.values.by_count = divisor(a.values.count);
 }
 
 size_t elem_size(int32_t dtype) { return dtype == CUSTOS_HIP_F32 ? 4 : 2; }
@@ -933,57 +1096,70 @@ struct Kernel {
     const char* name;
 };
 
-template <class T>
+// Kernels by plan, element type, activation, and whether x is a checkpoint.
+template <class T, int ACT>
 Kernel forward_tile(const Plan& p) {
     constexpr int V = VecOf<T>::elems;
     const char* name = "custos_group_norm_tile";
     const bool wide = p.vec > 1;
-    if (p.threads == 1024) return {wide ? handle(custos_group_norm_tile<T, V, 16, 1024>) : handle(custos_group_norm_tile<T, 1, 16, 1024>), name};
-    if (p.held == 16) return {wide ? handle(custos_group_norm_tile<T, V, 16, 256>) : handle(custos_group_norm_tile<T, 1, 16, 256>), name};
-    return {wide ? handle(custos_group_norm_tile<T, V, 4, 256>) : handle(custos_group_norm_tile<T, 1, 4, 256>), name};
+    if (!wide) {  // (rows of less than a vector, and rows that are no whole vectors in place)
+        if (p.threads == 256) return {handle(custos_group_norm_tile<T, 1, 8, 256, ACT>), name};
+        return {handle(custos_group_norm_tile<T, 1, 16, 1024, ACT>), name};
+    }
+    if (p.threads == 256) return {p.held == 4 ? handle(custos_group_norm_tile<T, V, 4, 256, ACT>) : handle(custos_group_norm_tile<T, V, 8, 256, ACT>), name};
+    if (p.held == 4) return {handle(custos_group_norm_tile<T, V, 4, 1024, ACT>), name};
+    return {p.held == 8 ? handle(custos_group_norm_tile<T, V, 8, 1024, ACT>) : handle(custos_group_norm_tile<T, V, 16, 1024, ACT>), name};
 }
 template <class T>
 Kernel forward_parts(const Plan& p) {
     constexpr int V = VecOf<T>::elems;
     return {p.vec > 1 ? handle(custos_group_norm_parts<T, V>) : handle(custos_group_norm_parts<T, 1>), "custos_group_norm_parts"};
 }
-template <class T>
+template <class T, int ACT>
 Kernel forward_values(const Plan& p) {
     constexpr int V = VecOf<T>::elems;
-    return {p.vec > 1 ? handle(custos_group_norm_values<T, V>) : handle(custos_group_norm_values<T, 1>), "custos_group_norm_values"};
+    const char* name = "custos_group_norm_values";
+    if (p.vec == 1) return {handle(custos_group_norm_values<T, 1, ACT, false>), name};
+    return {p.stream ? handle(custos_group_norm_values<T, V, ACT, true>) : handle(custos_group_norm_values<T, V, ACT, false>), name};
 }
-template <class T, bool SAVED>
+template <class T, int ACT, bool SAVED>
 Kernel backward_tile(const Plan& p) {
     constexpr int V = VecOf<T>::elems;
     const char* name = "custos_group_norm_grad_tile";
     const bool wide = p.vec > 1;
     if (p.threads == 1024)
-        return {wide ? handle(custos_group_norm_grad_tile<T, V, 4, 1024, SAVED>) : handle(custos_group_norm_grad_tile<T, 1, 4, 1024, SAVED>), name};
-    return {wide ? handle(custos_group_norm_grad_tile<T, V, 4, 256, SAVED>) : handle(custos_group_norm_grad_tile<T, 1, 4, 256, SAVED>), name};
+        return {wide ? handle(custos_group_norm_grad_tile<T, V, 4, 1024, SAVED, ACT>) : handle(custos_group_norm_grad_tile<T, 1, 4, 1024, SAVED, ACT>), name};
+    return {wide ? handle(custos_group_norm_grad_tile<T, V, 4, 256, SAVED, ACT>) : handle(custos_group_norm_grad_tile<T, 1, 4, 256, SAVED, ACT>), name};
 }
-template <class T, bool SAVED>
+template <class T, int ACT, bool SAVED>
 Kernel backward_parts(const Plan& p) {
     constexpr int V = VecOf<T>::elems;
-    return {p.vec > 1 ? handle(custos_group_norm_grad_parts<T, V, SAVED>) : handle(custos_group_norm_grad_parts<T, 1, SAVED>),
+    return {p.vec > 1 ? handle(custos_group_norm_grad_parts<T, V, SAVED, ACT>) : handle(custos_group_norm_grad_parts<T, 1, SAVED, ACT>),
             "custos_group_norm_grad_parts"};
 }
-template <class T, bool SAVED>
+template <class T, int ACT, bool SAVED>
 Kernel backward_values(const Plan& p) {
     constexpr int V = VecOf<T>::elems;
-    return {p.vec > 1 ? handle(custos_group_norm_grad_values<T, V, SAVED>) : handle(custos_group_norm_grad_values<T, 1, SAVED>),
-            "custos_group_norm_grad_values"};
-}
-template <class T>
-Kernel backward_sums() {
-    return {handle(custos_group_norm_grad_sums<T>), "custos_group_norm_grad_sums"};
+    const char* name = "custos_group_norm_grad_values";
+    if (p.vec == 1) return {handle(custos_group_norm_grad_values<T, 1, SAVED, ACT, false>), name};
+    return {p.stream ? handle(custos_group_norm_grad_values<T, V, SAVED, ACT, true>) : handle(custos_group_norm_grad_values<T, V, SAVED, ACT, false>), name};
 }
 
-// `pick<T>()` for the element type
+// `pick(element type, activation)`
+template <class T, class F>
+Kernel by_activation(int32_t activation, F pick) {
+    switch (activation) {
+        case CUSTOS_HIP_ACT_RELU: return pick(T(), std::integral_constant<int, kRelu>());
+        case CUSTOS_HIP_ACT_SILU: return pick(T(), std::integral_constant<int, kSilu>());
+        case CUSTOS_HIP_ACT_GELU: return pick(T(), std::integral_constant<int, kGelu>());
+        default: return pick(T(), std::integral_constant<int, kNone>());
+    }
+}
 template <class F>
-Kernel by_type(int32_t dtype, F pick) {
-    if (dtype == CUSTOS_HIP_F32) return pick(float());
-    if (dtype == CUSTOS_HIP_F16) return pick(static_cast<_Float16>(0));
-    return pick(static_cast<__bf16>(0));
+Kernel kernel_for(const custos_hip_group_norm_desc& d, F pick) {
+    if (d.dtype == CUSTOS_HIP_F32) return by_activation<float>(d.activation, pick);
+    if (d.dtype == CUSTOS_HIP_F16) return by_activation<_Float16>(d.activation, pick);
+    return by_activation<__bf16>(d.activation, pick);
 }
 
 int32_t launch(custos_hip_device* dev, const Kernel& k, u64 blocks, int threads, const GroupNormArgs& a, const Access* acc, size_t n_acc) {
@@ -1030,7 +1206,7 @@ int32_t custos_hip_group_norm(custos_hip_device* dev, const custos_hip_group_nor
     REQUIRE_DEV(dev);
 
     Plan plan;
-    make_plan(*desc, es, kForwardHeld, &plan);
+    make_plan(*desc, es, 2 * rows * desc->channels * es, /*accumulates=*/false, kForwardHeld, &plan);
     GroupNormArgs& a = plan.a;
     a.x = reinterpret_cast<const void*>(x);
     a.gamma = reinterpret_cast<const void*>(gamma);
@@ -1042,27 +1218,25 @@ int32_t custos_hip_group_norm(custos_hip_device* dev, const custos_hip_group_nor
     a.param_f32 = desc->param_dtype == CUSTOS_HIP_F32;
     Access acc[6];
     for (size_t i = 0; i < n; i++) acc[i] = ops[i].access();
-    const u64 parts = static_cast<u64>(a.samples) * a.splits, blocks = parts * a.tiles;
-    rc = check_grid(dev, "group norm", blocks);
+    const u64 parts = static_cast<u64>(a.samples) * a.parts.count, blocks = parts * a.tiles;
+    rc = check_grid(dev, "group norm", std::max<u64>(blocks, static_cast<u64>(a.samples) * a.tiles * a.values.count));
     if (rc != CUSTOS_HIP_OK) return rc;
     if (plan.in_registers)
-        return launch(dev, by_type(desc->dtype, [&](auto t) { return forward_tile<decltype(t)>(plan); }), blocks, plan.threads, a, acc, n);
+        return launch(dev, kernel_for(*desc, [&](auto t, auto act) { return forward_tile<decltype(t), act.value>(plan); }), blocks, plan.threads, a, acc, n);
 
-    const size_t bytes = parts * a.groups * 2 * sizeof(float);
+    const size_t part_bytes = parts * a.groups * 2 * sizeof(float);
     uint64_t area = 0;
-    rc = operator_workspace(dev, bytes, &area);
+    rc = operator_workspace(dev, part_bytes, &area);
     if (rc != CUSTOS_HIP_OK) return rc;
-    a.partial = reinterpret_cast<float*>(area);
-    const Access area_written{area, area + bytes, true}, area_read{area, area + bytes, false};
-    const Access in_parts[2] = {ops[2].access(), area_written};
-    rc = launch(dev, by_type(desc->dtype, [&](auto t) { return forward_parts<decltype(t)>(plan); }), blocks, kBlock, a, in_parts, 2);
+    a.group_parts = reinterpret_cast<float*>(area);
+    const Access in_parts[2] = {ops[2].access(), {area, area + part_bytes, true}};
+    acc[n] = {area, area + part_bytes, false};
+    rc = launch(dev, kernel_for(*desc, [&](auto t, auto) { return forward_parts<decltype(t)>(plan); }), blocks, kBlock, a, in_parts, 2);
     if (rc != CUSTOS_HIP_OK) return rc;
-    const Access in_stats[2] = {area_read, ops[1].access()};
-    const u64 waves = static_cast<u64>(a.samples) * a.groups;
-    rc = launch(dev, {handle(custos_group_norm_stats), "custos_group_norm_stats"}, (waves + kBlock / 64 - 1) / (kBlock / 64), kBlock, a, in_stats, 2);
-    if (rc != CUSTOS_HIP_OK) return rc;
-    acc[1].write = false;  // (the values read the statistics)
-    return launch(dev, by_type(desc->dtype, [&](auto t) { return forward_values<decltype(t)>(plan); }), blocks, kBlock, a, acc, n);
+    if (out == x) narrow_values(&plan);
+    a.blocks = static_cast<unsigned int>(static_cast<u64>(a.samples) * a.tiles * a.values.count);
+    return launch(dev, kernel_for(*desc, [&](auto t, auto act) { return forward_values<decltype(t), act.value>(plan); }), a.blocks, kBlock, a, acc,
+                  n + 1);
 }
 
 int32_t custos_hip_add_group_norm_grad(custos_hip_device* dev, const custos_hip_group_norm_desc* desc, uint64_t x, uint64_t x_pitch,
@@ -1108,7 +1282,8 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device* dev, const custos_hip_
     if (first_read == 0) return CUSTOS_HIP_OK;  // no gradient is wanted
 
     Plan plan;
-    make_plan(*desc, es, kBackwardHeld, &plan);
+    make_plan(*desc, es, total * (saved ? 2 * es + 1 : 3 * es),
+              /*accumulates=*/!overwrite, kBackwardHeld, &plan);
     GroupNormArgs& a = plan.a;
     a.x = reinterpret_cast<const void*>(x);
     a.codes = reinterpret_cast<const signed char*>(codes);
@@ -1123,62 +1298,52 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device* dev, const custos_hip_
     a.out_pitch = x_grad_pitch;
     a.param_f32 = desc->param_dtype == CUSTOS_HIP_F32;
     a.accumulate = !overwrite;
-    const u64 parts = static_cast<u64>(a.samples) * a.splits, blocks = parts * a.tiles;
-    rc = check_grid(dev, what, std::max<u64>(blocks, static_cast<u64>(a.samples) * a.groups));
+    const u64 parts = static_cast<u64>(a.samples) * a.parts.count, blocks = parts * a.tiles;
+    rc = check_grid(dev, what, std::max<u64>(blocks, static_cast<u64>(a.samples) * a.tiles * a.values.count) + a.channels);
     if (rc != CUSTOS_HIP_OK) return rc;
-    const size_t part_bytes = parts * 2 * a.channels * sizeof(float), sum_bytes = static_cast<size_t>(a.samples) * a.groups * 2 * sizeof(float);
+    const size_t channel_bytes = parts * 2 * a.channels * sizeof(float), part_bytes = parts * a.groups * 2 * sizeof(float);
+    const size_t area_bytes = channel_bytes + part_bytes;
     uint64_t area = 0;
-    rc = operator_workspace(dev, part_bytes + sum_bytes, &area);
+    rc = operator_workspace(dev, area_bytes, &area);
     if (rc != CUSTOS_HIP_OK) return rc;
-    a.partial = reinterpret_cast<float*>(area);
-    a.sums = reinterpret_cast<float*>(area + part_bytes);
-    const Access area_written{area, area + part_bytes + sum_bytes, true}, area_read{area, area + part_bytes + sum_bytes, false};
-    Access acc[10];
-    size_t n_acc = 0;
-    for (size_t i = first_read; i < n; i++) acc[n_acc++] = ops[i].access();
-    if (plan.in_registers) {
-        for (size_t i = 0; i < values_written; i++) acc[n_acc++] = ops[i].access();
-        acc[n_acc++] = area_written;
-        rc = launch(dev, by_type(desc->dtype, [&](auto t) { return saved ? backward_tile<decltype(t), true>(plan) : backward_tile<decltype(t), false>(plan); }),
-                    blocks, plan.threads, a, acc, n_acc);
-        if (rc != CUSTOS_HIP_OK) return rc;
-    } else {
-        acc[n_acc] = area_written;
-        rc = launch(dev, by_type(desc->dtype, [&](auto t) { return saved ? backward_parts<decltype(t), true>(plan) : backward_parts<decltype(t), false>(plan); }),
-                    blocks, kBlock, a, acc, n_acc + 1);
-        if (rc != CUSTOS_HIP_OK) return rc;
-        Access in_sums[2] = {area_written, {}};
-        size_t n_sums = 1;
-        if (gamma) in_sums[n_sums++] = {gamma, gamma + desc->channels * ps, false};
-        rc = launch(dev, by_type(desc->dtype, [&](auto t) { return backward_sums<decltype(t)>(); }), static_cast<u64>(a.samples) * a.groups,
-                    kBlock, a, in_sums, n_sums);
-        if (rc != CUSTOS_HIP_OK) return rc;
-        if (x_grad) {
-            acc[n_acc++] = area_read;
-            acc[n_acc++] = ops[0].access();
-            rc = launch(dev, by_type(desc->dtype, [&](auto t) { return saved ? backward_values<decltype(t), true>(plan) : backward_values<decltype(t), false>(plan); }),
-                        blocks, kBlock, a, acc, n_acc);
-            if (rc != CUSTOS_HIP_OK) return rc;
-        }
-    }
-    if (!gamma_grad && !beta_grad) return CUSTOS_HIP_OK;
-    const u64 stride = static_cast<u64>(a.splits) * 2 * a.channels;
-    const float* sums = a.partial;
-    float *dgamma = reinterpret_cast<float*>(gamma_grad), *dbeta = reinterpret_cast<float*>(beta_grad);
-    const OpArg args[] = {{&sums, 8}, {&stride, 8}, {&a.samples, 4}, {&a.channels, 4}, {&dgamma, 8}, {&dbeta, 8}, {&a.accumulate, 4}};
+    a.group_parts = reinterpret_cast<float*>(area);
+    a.channel_parts = reinterpret_cast<float*>(area + part_bytes);
+    a.gamma_grad = reinterpret_cast<float*>(gamma_grad);
+    a.beta_grad = reinterpret_cast<float*>(beta_grad);
+    const Access area_written{area, area + area_bytes, true}, area_read{area, area + area_bytes, false};
+    // what every launch reads, then what it writes
+    Access acc[12];
+    size_t n_read = 0;
+    for (size_t i = first_read; i < n; i++) acc[n_read++] = ops[i].access();
+    const u64 param_blocks = gamma_grad || beta_grad ? (a.channels + kParamChannels - 1) / kParamChannels : 0;
     Access in_params[3] = {area_read, {}, {}};
     size_t n_params = 1;
     for (size_t i = values_written; i < first_read; i++) in_params[n_params++] = ops[i].access();
-    OpLaunch op{};
-    op.name = "custos_group_norm_param_grads";
-    op.func = handle(custos_group_norm_param_grads);
-    op.grid = dim3((a.channels + kBlock - 1) / kBlock);
-    op.block = dim3(kBlock);
-    op.args = args;
-    op.n_args = sizeof args / sizeof args[0];
-    op.acc = in_params;
-    op.n_acc = n_params;
-    return launch_op(dev, op);
+    if (plan.in_registers || !x_grad) {
+        size_t n_acc = n_read;
+        if (plan.in_registers && x_grad) acc[n_acc++] = ops[0].access();
+        acc[n_acc++] = area_written;
+        rc = launch(dev, kernel_for(*desc, [&](auto t, auto act) {
+                        using T = decltype(t);
+                        constexpr int ACT = act.value;
+                        if (plan.in_registers) return saved ? backward_tile<T, ACT, true>(plan) : backward_tile<T, ACT, false>(plan);
+                        return saved ? backward_parts<T, ACT, true>(plan) : backward_parts<T, ACT, false>(plan);
+                    }), blocks, plan.threads, a, acc, n_acc);
+        if (rc != CUSTOS_HIP_OK || param_blocks == 0) return rc;
+        return launch(dev, {handle(custos_group_norm_param_grads), "custos_group_norm_param_grads"}, param_blocks, kBlock, a, in_params, n_params);
+    }
+    acc[n_read] = area_written;
+    rc = launch(dev, kernel_for(*desc, [&](auto t, auto act) { return saved ? backward_parts<decltype(t), act.value, true>(plan) : backward_parts<decltype(t), act.value, false>(plan); }),
+                blocks, kBlock, a, acc, n_read + 1);
+    if (rc != CUSTOS_HIP_OK) return rc;
+    size_t n_acc = n_read;
+    acc[n_acc++] = area_read;
+    acc[n_acc++] = ops[0].access();
+    for (size_t i = 1; i < n_params; i++) acc[n_acc++] = in_params[i];
+    if (!overwrite || x_grad == x || x_grad == out_grad) narrow_values(&plan);
+    a.blocks = static_cast<unsigned int>(static_cast<u64>(a.samples) * a.tiles * a.values.count);
+    return launch(dev, kernel_for(*desc, [&](auto t, auto act) { return saved ? backward_values<decltype(t), act.value, true>(plan) : backward_values<decltype(t), act.value, false>(plan); }),
+                  a.blocks + param_blocks, kBlock, a, acc, n_acc);
 }
 
 }  // extern "C"

@@ -71,6 +71,42 @@ __device__ __forceinline__ T from_f32(float x) {
     return static_cast<T>(x);
 }
 
+// Makes the compiler forget what it knows of a held value, so that it converts the stored bits again where
+// they are used next instead of keeping the converted values, which take twice the registers or more.
+__device__ __forceinline__ void forget(u32x4& v) {
+    unsigned int a = v[0], b = v[1], c = v[2], d = v[3];
+    __asm__("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+    v = u32x4{a, b, c, d};
+}
+__device__ __forceinline__ void forget(u32x2& v) {
+    unsigned int a = v[0], b = v[1];
+    __asm__("" : "+v"(a), "+v"(b));
+    v = u32x2{a, b};
+}
+__device__ __forceinline__ void forget(unsigned int& v) { __asm__("" : "+v"(v)); }
+__device__ __forceinline__ void forget(unsigned short&) {}
+__device__ __forceinline__ void forget(unsigned char&) {}
+
+// A vector as it is stored.
+template <class T, int V>
+struct Bits {
+    using Storage = typename Raw<V * sizeof(T), sizeof(T)>::base;
+    Storage bits;
+    // STREAM: past the caches (what is not read again soon)
+    template <bool STREAM = false>
+    __device__ __forceinline__ void load(const T* p) {
+        using Any = typename Raw<V * sizeof(T), sizeof(T)>::type;
+        if (STREAM) bits = __builtin_nontemporal_load(reinterpret_cast<const Any*>(p));
+        else bits = *reinterpret_cast<const Any*>(p);
+    }
+    __device__ __forceinline__ void zero() { bits = Storage(0); }
+    __device__ __forceinline__ void forget_values() { forget(bits); }
+    __device__ __forceinline__ Pack<T, V> pack() const {
+        using Out = Pack<T, V>;
+        return __builtin_bit_cast(Out, bits);
+    }
+};
+
 // Sum over the aligned groups of `WIDTH` lanes of a wavefront, in every lane (a fixed tree: results do not
 // depend on timing).
 template <int WIDTH>
