@@ -38,7 +38,7 @@ struct RowArgs {
     void* grad;             // null: not wanted
     float* logp;
     float* lse;             // log-probabilities only; may be null
-    double* terms;          // policy: [rows][4], the four totals' parts; null: not wanted
+    float4* terms;          // policy: [rows], the four totals' parts; null: not wanted
     u64 pitch, grad_pitch;
     unsigned int vocab;
     float inv_t, scale2;    // 1 / T, log2(e) / T
@@ -74,7 +74,7 @@ struct Running {
 };
 
 // A vector of a row: V elements from `first` on.  The last one starts at vocab - V, and its first `dup`
-// elements are also the vector before it's.
+// elements are also the vector before it's: not summed twice, and stored twice with the same value.
 template <int V>
 struct Place {
     unsigned int first;
@@ -95,18 +95,7 @@ __device__ __forceinline__ void add_vector(Running* run, const Pack<T, V>& p, in
     run->add(z, scale2);
 }
 
-template <class T, int V>
-__device__ __forceinline__ void put(T* row, const Place<V>& at, const Pack<T, V>& p) {
-    if (at.dup == 0) {
-        store_pack<false, T, V>(row + at.first, p);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; j++)
-            if (j >= at.dup) row[at.first + j] = p.v[j];
-    }
-}
-
-// What the gradient's elements need: dz = e * factor, + slope at the label.
+// What the gradient's elements need: dz = exp * factor, + slope at the label.
 struct RowGradient {
     float base, factor, slope;
     int label;
@@ -127,22 +116,28 @@ struct RowGradient {
     }
 };
 
-// The few values of a row, by one whole wavefront; lane 0 writes them down.  `z_label`: the label's logit.
+// What a row brings besides its logits.
+struct RowInputs {
+    int label;
+    float z_label, weight, advantage, old_logp, ref_logp;
+};
+
+// The few values of a row, by one whole wavefront; lane 0 writes them down.
 template <int MODE>
-__device__ __forceinline__ void finish_row(const RowArgs& a, u64 row, int label, const Running& run, float z_label, RowGradient* out) {
+__device__ __forceinline__ void finish_row(const RowArgs& a, u64 row, const RowInputs& in, const Running& run, RowGradient* out) {
     const unsigned int lane = threadIdx.x % 64;
     const double log_sum = log(static_cast<double>(run.sum));
     const double inv_t = static_cast<double>(a.inv_t);
-    const bool chosen = label >= 0;
-    const double logp = (static_cast<double>(z_label) - static_cast<double>(run.max)) * inv_t - log_sum;
+    const bool chosen = in.label >= 0;
+    const double logp = (static_cast<double>(in.z_label) - static_cast<double>(run.max)) * inv_t - log_sum;
     if (lane == 0 && a.logp) a.logp[row] = chosen ? static_cast<float>(logp) : 0.0f;
     if (MODE == kLogprob) {
         if (lane == 0 && a.lse) a.lse[row] = static_cast<float>(static_cast<double>(run.max) * inv_t + log_sum);
         return;
     }
-    const double weight = a.weights[row], advantage = a.advantages[row];
-    const double moved = logp - static_cast<double>(a.old_logp[row]);
-    const double behind = a.ref_logp ? static_cast<double>(a.ref_logp[row]) - logp : 0.0;
+    const double weight = in.weight, advantage = in.advantage;
+    const double moved = logp - static_cast<double>(in.old_logp);
+    const double behind = a.ref_logp ? static_cast<double>(in.ref_logp) - logp : 0.0;
     // exp - 1 of both differences at once, in two lanes
     const double em1 = expm1(lane == 0 ? moved : behind);
     const double ratio = __shfl(em1, 0, 64) + 1.0, behind_em1 = __shfl(em1, 1, 64);
@@ -151,22 +146,19 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, u64 row, int label,
     const double clipped = fmin(fmax(ratio, 1.0 - a.clip_low), 1.0 + a.clip_high) * advantage;
     const bool inside = !(plain > clipped);  // (a NaN stays one)
     const double value = inside ? plain : clipped;
-    if (lane == 0 && a.terms) {
-        double* t = a.terms + row * 4;
-        t[0] = weight * (a.kl_coef * kl - value);
-        t[1] = weight * kl;
-        t[2] = inside ? 0.0 : weight;
-        t[3] = weight * ratio;
-    }
+    if (lane == 0 && a.terms)
+        a.terms[row] = make_float4(static_cast<float>(weight * (a.kl_coef * kl - value)), static_cast<float>(weight * kl),
+                                   inside ? 0.0f : in.weight, static_cast<float>(weight * ratio));
     const double slope = weight * ((inside ? -plain : 0.0) - a.kl_coef * behind_em1) * a.grad_factor;
     out->base = Running::base(run.max);
     out->slope = static_cast<float>(slope);
     out->factor = static_cast<float>(-slope / static_cast<double>(run.sum));
-    out->label = label;
+    out->label = in.label;
 }
 
 // One workgroup per row.  HELD > 0: the row is held in registers, HELD vectors a thread; 0: it is read twice.
-template <class T, int V, int HELD, int THREADS, int MODE>
+// STREAM: the gradient is stored past the caches.
+template <class T, int V, int HELD, int THREADS, int MODE, bool STREAM>
 __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
     constexpr int kWaves = THREADS / 64;
     __shared__ float part_max[kWaves], part_sum[kWaves];
@@ -176,45 +168,59 @@ __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
     const T* z = static_cast<const T*>(a.logits) + row * a.pitch;
     T* grad = MODE == kPolicy && a.grad ? static_cast<T*>(a.grad) + row * a.grad_pitch : nullptr;
     const unsigned int vecs = (a.vocab + V - 1) / V;
-    const int label = a.labels[row];
-    // a row nothing is asked of is not read
-    if (MODE == kLogprob ? label < 0 && !a.lse : label < 0 || a.weights[row] == 0.0f) {
+    RowInputs in;
+    in.label = a.labels[row];
+    if (MODE == kPolicy) {  // (all of them now: nothing waits for them at the end)
+        in.weight = a.weights[row];
+        in.advantage = a.advantages[row];
+        in.old_logp = a.old_logp[row];
+        in.ref_logp = a.ref_logp ? a.ref_logp[row] : 0.0f;
+    }
+    // a row nothing is asked of is not read (but for its first quarter, which is under way when that is known)
+    constexpr int kFirst = HELD / 4;
+    Bits<T, V> held[HELD > 0 ? HELD : 1];
+    auto load_held = [&](int i) {
+        const unsigned int v = t + i * THREADS;
+        if (v < vecs) held[i].template load<true>(z + Place<V>(v, a.vocab).first);
+    };
+#pragma unroll
+    for (int i = 0; i < kFirst; i++) load_held(i);
+    if (MODE == kLogprob ? in.label < 0 && !a.lse : in.label < 0 || in.weight == 0.0f) {
         if (t == 0) {
             if (a.logp) a.logp[row] = 0.0f;
-            if (MODE == kPolicy && a.terms) a.terms[row * 4] = a.terms[row * 4 + 1] = a.terms[row * 4 + 2] = a.terms[row * 4 + 3] = 0.0;
+            if (MODE == kPolicy && a.terms) a.terms[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         if (grad) {
             Pack<T, V> zero;
 #pragma unroll
             for (int j = 0; j < V; j++) zero.v[j] = from_f32<T>(0.0f);
-            for (unsigned int v = t; v < vecs; v += THREADS) put<T, V>(grad, Place<V>(v, a.vocab), zero);
+            for (unsigned int v = t; v < vecs; v += THREADS) store_pack<STREAM, T, V>(grad + Place<V>(v, a.vocab).first, zero);
         }
         return;
     }
-    // (a label behind the vocabulary: NaN, and no read)
-    const float z_label = label < 0 ? 0.0f : static_cast<unsigned int>(label) < a.vocab ? to_f32(z[label]) : __builtin_nanf("");
     Running run;
-    Pack<T, V> held[HELD > 0 ? HELD : 1];
     if (HELD > 0) {
 #pragma unroll
-        for (int i = 0; i < HELD; i++) {
-            const unsigned int v = t + i * THREADS;
-            if (v < vecs) held[i] = load_pack<false, T, V>(z + Place<V>(v, a.vocab).first);
-        }
+        for (int i = kFirst; i < HELD; i++) load_held(i);
+        // (a label behind the vocabulary: NaN, and no read)
+        in.z_label = in.label < 0 ? 0.0f : static_cast<unsigned int>(in.label) < a.vocab ? to_f32(z[in.label]) : __builtin_nanf("");
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
             const unsigned int v = t + i * THREADS;
-            if (v < vecs) add_vector<T, V>(&run, held[i], Place<V>(v, a.vocab).dup, a.scale2);
+            if (v >= vecs) break;
+            add_vector<T, V>(&run, held[i].pack(), Place<V>(v, a.vocab).dup, a.scale2);
+            held[i].forget_values();
         }
     } else {
+        in.z_label = in.label < 0 ? 0.0f : static_cast<unsigned int>(in.label) < a.vocab ? to_f32(z[in.label]) : __builtin_nanf("");
         constexpr int kAhead = 4;
         unsigned int v = t;
         for (; v + (kAhead - 1) * THREADS < vecs - 1; v += kAhead * THREADS) {
-            Pack<T, V> p[kAhead];
+            Bits<T, V> p[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; u++) p[u] = load_pack<false, T, V>(z + (v + u * THREADS) * V);
+            for (int u = 0; u < kAhead; u++) p[u].load(z + (v + u * THREADS) * V);
 #pragma unroll
-            for (int u = 0; u < kAhead; u++) add_vector<T, V>(&run, p[u], 0, a.scale2);
+            for (int u = 0; u < kAhead; u++) add_vector<T, V>(&run, p[u].pack(), 0, a.scale2);
         }
         for (; v < vecs; v += THREADS) {
             const Place<V> at(v, a.vocab);
@@ -229,7 +235,7 @@ __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
         run.sum = t < kWaves ? part_sum[t] : 0.0f;
         run.join_lanes(a.scale2);
         RowGradient g;
-        finish_row<MODE>(a, row, label, run, z_label, &g);
+        finish_row<MODE>(a, row, in, run, &g);
         if (MODE == kPolicy && t == 0) shared = g;
     }
     if (MODE == kLogprob || !grad) return;
@@ -241,27 +247,34 @@ __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
             const unsigned int v = t + i * THREADS;
             if (v >= vecs) break;
             const Place<V> at(v, a.vocab);
-            put<T, V>(grad, at, g.of<T, V>(held[i], at.first, a.scale2));
+            store_pack<STREAM, T, V>(grad + at.first, g.of<T, V>(held[i].pack(), at.first, a.scale2));
         }
     } else {
         for (unsigned int v = t; v < vecs; v += THREADS) {
             const Place<V> at(v, a.vocab);
-            put<T, V>(grad, at, g.of<T, V>(load_pack<false, T, V>(z + at.first), at.first, a.scale2));
+            const Pack<T, V> y = g.of<T, V>(load_pack<false, T, V>(z + at.first), at.first, a.scale2);
+            if (at.dup == 0) {
+                store_pack<STREAM, T, V>(grad + at.first, y);
+            } else {  // (in place, the thread of the vector before may have stored its gradient over what was loaded here)
+                for (int j = at.dup; j < V; j++) grad[at.first + j] = y.v[j];
+            }
         }
     }
 }
 
-// Sums of rows of four, `rows_each` rows a workgroup, in a fixed order; to `sums` (f64), or, by one workgroup,
-// to `totals` (f32).
-constexpr int kSumThreads = 256;
-__global__ void __launch_bounds__(kSumThreads) custos_policy_totals(const double* terms, u64 rows, u64 rows_each, double* sums, float* totals) {
+// Sums of rows of four, `rows_each` rows a workgroup, in a fixed order and in f64; to `sums`, of which the next launch
+// adds up 8192 again.
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads) custos_policy_totals(const float4* terms, u64 rows, u64 rows_each, float4* sums) {
     __shared__ double parts[kSumThreads / 64][4];
     const unsigned int t = threadIdx.x;
     const u64 begin = blockIdx.x * rows_each, end = min(begin + rows_each, rows);
     double s[4] = {0.0, 0.0, 0.0, 0.0};
-    for (u64 r = begin + t; r < end; r += kSumThreads)
-#pragma unroll
-        for (int k = 0; k < 4; k++) s[k] += terms[r * 4 + k];
+#pragma unroll 4
+    for (u64 r = begin + t; r < end; r += kSumThreads) {
+        const float4 v = terms[r];
+        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+    }
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         s[k] = lanes_sum_f64(s[k]);
@@ -271,39 +284,45 @@ __global__ void __launch_bounds__(kSumThreads) custos_policy_totals(const double
     if (t >= 4) return;
     double total = 0.0;
     for (int w = 0; w < kSumThreads / 64; w++) total += parts[w][t];
-    if (totals) totals[t] = static_cast<float>(total);
-    else sums[blockIdx.x * 4 + t] = total;
+    reinterpret_cast<float*>(sums + blockIdx.x)[t] = static_cast<float>(total);
 }
 
 // ---- host ----
+
+constexpr u64 kStreamBeyond = 64ull << 20;
 
 struct Kernel {
     void* fn;
     int threads;
 };
 
-template <class T, int V, int MODE>
+template <class T, int V, int MODE, bool STREAM>
 Kernel kernel_for(unsigned int vocab) {
     const u64 vecs = (static_cast<u64>(vocab) + V - 1) / V;
 #define CUSTOS_ROWS(HELD, THREADS) \
-    if (HELD == 0 || vecs <= static_cast<u64>(HELD) * THREADS) return {reinterpret_cast<void*>(custos_policy_rows<T, V, HELD, THREADS, MODE>), THREADS}
+    if (HELD == 0 || vecs <= static_cast<u64>(HELD) * THREADS) return {reinterpret_cast<void*>(custos_policy_rows<T, V, HELD, THREADS, MODE, STREAM>), THREADS}
     CUSTOS_ROWS(4, 64);
     CUSTOS_ROWS(4, 256);
     CUSTOS_ROWS(16, 256);
-    CUSTOS_ROWS(8, 1024);
+    CUSTOS_ROWS(16, 512);
     CUSTOS_ROWS(16, 1024);
     CUSTOS_ROWS(0, 1024);
 #undef CUSTOS_ROWS
 }
 
-template <int MODE>
-Kernel kernel_of(int32_t dtype, unsigned int vocab) {
+template <class T, int MODE>
+Kernel kernel_of_type(unsigned int vocab, bool stream) {
+    constexpr int V = VecOf<T>::elems;
     // (a row shorter than a vector: element by element)
-    if (dtype == CUSTOS_HIP_F32)
-        return vocab >= 4 ? kernel_for<float, 4, MODE>(vocab) : Kernel{reinterpret_cast<void*>(custos_policy_rows<float, 1, 4, 64, MODE>), 64};
-    if (dtype == CUSTOS_HIP_F16)
-        return vocab >= 8 ? kernel_for<_Float16, 8, MODE>(vocab) : Kernel{reinterpret_cast<void*>(custos_policy_rows<_Float16, 1, 4, 64, MODE>), 64};
-    return vocab >= 8 ? kernel_for<__bf16, 8, MODE>(vocab) : Kernel{reinterpret_cast<void*>(custos_policy_rows<__bf16, 1, 4, 64, MODE>), 64};
+    if (vocab < static_cast<unsigned int>(V)) return {reinterpret_cast<void*>(custos_policy_rows<T, 1, 1, 64, MODE, false>), 64};
+    if (MODE == kPolicy && stream) return kernel_for<T, V, kPolicy, true>(vocab);
+    return kernel_for<T, V, MODE, false>(vocab);
+}
+template <int MODE>
+Kernel kernel_of(int32_t dtype, unsigned int vocab, bool stream) {
+    if (dtype == CUSTOS_HIP_F32) return kernel_of_type<float, MODE>(vocab, stream);
+    if (dtype == CUSTOS_HIP_F16) return kernel_of_type<_Float16, MODE>(vocab, stream);
+    return kernel_of_type<__bf16, MODE>(vocab, stream);
 }
 
 size_t elem_size(int32_t dtype) { return dtype == CUSTOS_HIP_F32 ? 4 : 2; }
@@ -336,19 +355,16 @@ int32_t launch(custos_hip_device* dev, const char* name, void* fn, u64 blocks, i
 
 constexpr u64 kRowsEach = 8192;  // rows a workgroup of the totals adds up
 
-int32_t launch_totals(custos_hip_device* dev, uint64_t terms, u64 rows, uint64_t area_end, uint64_t totals) {
+int32_t launch_totals(custos_hip_device* dev, uint64_t terms, u64 rows, uint64_t totals) {
     while (true) {
-        const u64 blocks = (rows + kRowsEach - 1) / kRowsEach;
-        const bool last = blocks <= 1;
-        const uint64_t sums = last ? 0 : area_end - blocks * 32;  // (behind the rows they are the sums of)
-        const uint64_t out = last ? totals : 0;
-        const OpArg args[] = {{&terms, 8}, {&rows, 8}, {&kRowsEach, 8}, {&sums, 8}, {&out, 8}};
-        const Access acc[2] = {{terms, terms + rows * 32, false}, last ? Access{totals, totals + 16, true} : Access{sums, sums + blocks * 32, true}};
-        int32_t rc = launch(dev, "custos_policy_totals", reinterpret_cast<void*>(custos_policy_totals), blocks ? blocks : 1, kSumThreads, args, 5, acc, 2);
-        if (rc != CUSTOS_HIP_OK || last) return rc;
+        const u64 blocks = std::max<u64>(1, (rows + kRowsEach - 1) / kRowsEach);
+        const uint64_t sums = blocks == 1 ? totals : terms + rows * sizeof(float4);  // (behind the rows they are the sums of)
+        const OpArg args[] = {{&terms, 8}, {&rows, 8}, {&kRowsEach, 8}, {&sums, 8}};
+        const Access acc[2] = {{terms, terms + rows * sizeof(float4), false}, {sums, sums + blocks * sizeof(float4), true}};
+        int32_t rc = launch(dev, "custos_policy_totals", reinterpret_cast<void*>(custos_policy_totals), blocks, kSumThreads, args, 4, acc, 2);
+        if (rc != CUSTOS_HIP_OK || blocks == 1) return rc;
         terms = sums;
         rows = blocks;
-        area_end = sums;
     }
 }
 
@@ -389,7 +405,7 @@ int32_t custos_hip_token_logprob(custos_hip_device* dev, int32_t dtype, uint64_t
     a.scale2 = static_cast<float>(1.4426950408889634 / temperature);
     Access acc[4];
     for (size_t i = 0; i < n; i++) acc[i] = ops[i].access();
-    const Kernel k = kernel_of<kLogprob>(dtype, a.vocab);
+    const Kernel k = kernel_of<kLogprob>(dtype, a.vocab, false);
     const OpArg arg{&a, sizeof a};
     return launch(dev, "custos_token_logprob", k.fn, rows, k.threads, &arg, 1, acc, n);
 }
@@ -452,19 +468,19 @@ int32_t custos_hip_policy_loss(custos_hip_device* dev, const custos_hip_policy_d
     size_t n_acc = 0;
     for (size_t i = 0; i < without_totals; i++) acc[n_acc++] = ops[i].access();
     uint64_t area = 0;
-    // (the rows' parts, and the sums of 8192 of them each)
-    const size_t area_bytes = totals ? rows * 32 + (rows / kRowsEach + 64) * 64 : 0;
+    // (the rows' parts, and behind them the sums of 8192 of them each, and so on)
+    const size_t area_bytes = (rows + rows / (kRowsEach / 2) + 64) * sizeof(float4);
     if (totals) {
         rc = operator_workspace(dev, area_bytes, &area);
         if (rc != CUSTOS_HIP_OK) return rc;
-        a.terms = reinterpret_cast<double*>(area);
-        acc[n_acc++] = {area, area + rows * 32, true};
+        a.terms = reinterpret_cast<float4*>(area);
+        acc[n_acc++] = {area, area + rows * sizeof(float4), true};
     }
-    const Kernel k = kernel_of<kPolicy>(desc->dtype, a.vocab);
+    const Kernel k = kernel_of<kPolicy>(desc->dtype, a.vocab, 2 * rows * desc->vocab * es > kStreamBeyond);
     const OpArg arg{&a, sizeof a};
     rc = launch(dev, "custos_policy_rows", k.fn, rows, k.threads, &arg, 1, acc, n_acc);
     if (rc != CUSTOS_HIP_OK || !totals) return rc;
-    return launch_totals(dev, area, rows, area + area_bytes, totals);
+    return launch_totals(dev, area, rows, totals);
 }
 
 }  // extern "C"
