@@ -58,9 +58,14 @@ struct Running {
 #pragma unroll
         for (int j = 0; j < V; j++) m = fmaxf(m, z[j]);
         const float b = base(m);
-        sum *= __builtin_amdgcn_exp2f((max - b) * scale2);
+        float e[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) sum += __builtin_amdgcn_exp2f((z[j] - b) * scale2);
+        for (int j = 0; j < V; j++) e[j] = __builtin_amdgcn_exp2f((z[j] - b) * scale2);
+#pragma unroll
+        for (int half = V / 2; half > 0; half /= 2)
+#pragma unroll
+            for (int j = 0; j < half; j++) e[j] += e[j + half];
+        sum = sum * __builtin_amdgcn_exp2f((max - b) * scale2) + e[0];
         max = m;
     }
     // over the wavefront, in every lane
@@ -73,25 +78,25 @@ struct Running {
     }
 };
 
-// A vector of a row: V elements from `first` on.  The last one starts at vocab - V, and its first `dup`
-// elements are also the vector before it's: not summed twice, and stored twice with the same value.
-template <int V>
-struct Place {
-    unsigned int first;
-    int dup;
-    __device__ __forceinline__ Place(unsigned int vec, unsigned int vocab) : first(vec * V), dup(0) {
-        if (first + V > vocab) {
-            dup = static_cast<int>(first + V - vocab);
-            first = vocab - V;
-        }
+// The fewer than V elements of a row before the first 16-byte boundary, or behind the last whole vector: thread 0 has
+// the former, the last thread the latter, every other thread none.  What is not there counts as -inf.
+template <class T, int V>
+struct Edge {
+    unsigned int first = 0, count = 0;
+    T v[V];
+    __device__ __forceinline__ void load(const T* row) {
+        if (count == 0) return;
+#pragma unroll
+        for (int j = 0; j < V - 1; j++) v[j] = static_cast<unsigned int>(j) < count ? row[first + j] : from_f32<T>(-__builtin_inff());
+        v[V - 1] = from_f32<T>(-__builtin_inff());
     }
 };
 
 template <class T, int V>
-__device__ __forceinline__ void add_vector(Running* run, const Pack<T, V>& p, int dup, float scale2) {
+__device__ __forceinline__ void add_vector(Running* run, const Pack<T, V>& p, float scale2) {
     float z[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) z[j] = j >= dup ? to_f32(p.v[j]) : -__builtin_inff();
+    for (int j = 0; j < V; j++) z[j] = to_f32(p.v[j]);
     run->add(z, scale2);
 }
 
@@ -167,7 +172,12 @@ __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
     const u64 row = blockIdx.x;
     const T* z = static_cast<const T*>(a.logits) + row * a.pitch;
     T* grad = MODE == kPolicy && a.grad ? static_cast<T*>(a.grad) + row * a.grad_pitch : nullptr;
-    const unsigned int vecs = (a.vocab + V - 1) / V;
+    // whole vectors at 16-byte boundaries, from element `head` on, and the edges
+    const unsigned int head = min(a.vocab, static_cast<unsigned int>((16 - (reinterpret_cast<u64>(z) & 15)) & 15) / static_cast<unsigned int>(sizeof(T)));
+    const unsigned int vecs = (a.vocab - head) / V;
+    Edge<T, V> edge;
+    if (t == 0) edge.count = head;
+    if (t == THREADS - 1) edge.first = head + vecs * V, edge.count = a.vocab - edge.first;
     RowInputs in;
     in.label = a.labels[row];
     if (MODE == kPolicy) {  // (all of them now: nothing waits for them at the end)
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
     Bits<T, V> held[HELD > 0 ? HELD : 1];
     auto load_held = [&](int i) {
         const unsigned int v = t + i * THREADS;
-        if (v < vecs) held[i].template load<true>(z + Place<V>(v, a.vocab).first);
+        if (v < vecs) held[i].template load<true>(z + head + v * V);
     };
 #pragma unroll
     for (int i = 0; i < kFirst; i++) load_held(i);
@@ -194,39 +204,41 @@ __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
             Pack<T, V> zero;
 #pragma unroll
             for (int j = 0; j < V; j++) zero.v[j] = from_f32<T>(0.0f);
-            for (unsigned int v = t; v < vecs; v += THREADS) store_pack<STREAM, T, V>(grad + Place<V>(v, a.vocab).first, zero);
+            for (unsigned int v = t; v < vecs; v += THREADS) store_pack<STREAM, T, V>(grad + head + v * V, zero);
+            for (unsigned int j = 0; j < edge.count; j++) grad[edge.first + j] = zero.v[0];
         }
         return;
     }
+    // (a label behind the vocabulary: NaN, and no read)
+    in.z_label = in.label < 0 ? 0.0f : static_cast<unsigned int>(in.label) < a.vocab ? to_f32(z[in.label]) : __builtin_nanf("");
     Running run;
     if (HELD > 0) {
 #pragma unroll
         for (int i = kFirst; i < HELD; i++) load_held(i);
-        // (a label behind the vocabulary: NaN, and no read)
-        in.z_label = in.label < 0 ? 0.0f : static_cast<unsigned int>(in.label) < a.vocab ? to_f32(z[in.label]) : __builtin_nanf("");
+        edge.load(z);
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
-            const unsigned int v = t + i * THREADS;
-            if (v >= vecs) break;
-            add_vector<T, V>(&run, held[i].pack(), Place<V>(v, a.vocab).dup, a.scale2);
+            if (t + i * THREADS >= vecs) break;
+            add_vector<T, V>(&run, held[i].pack(), a.scale2);
             held[i].forget_values();
         }
     } else {
-        in.z_label = in.label < 0 ? 0.0f : static_cast<unsigned int>(in.label) < a.vocab ? to_f32(z[in.label]) : __builtin_nanf("");
+        edge.load(z);
         constexpr int kAhead = 4;
         unsigned int v = t;
-        for (; v + (kAhead - 1) * THREADS < vecs - 1; v += kAhead * THREADS) {
+        for (; v + (kAhead - 1) * THREADS < vecs; v += kAhead * THREADS) {
             Bits<T, V> p[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; u++) p[u].load(z + (v + u * THREADS) * V);
+            for (int u = 0; u < kAhead; u++) p[u].load(z + head + (v + u * THREADS) * V);
 #pragma unroll
-            for (int u = 0; u < kAhead; u++) add_vector<T, V>(&run, p[u].pack(), 0, a.scale2);
+            for (int u = 0; u < kAhead; u++) add_vector<T, V>(&run, p[u].pack(), a.scale2);
         }
-        for (; v < vecs; v += THREADS) {
-            const Place<V> at(v, a.vocab);
-            add_vector<T, V>(&run, load_pack<false, T, V>(z + at.first), at.dup, a.scale2);
-        }
+        for (; v < vecs; v += THREADS) add_vector<T, V>(&run, load_pack<false, T, V>(z + head + v * V), a.scale2);
     }
+    Pack<T, V> edge_values;
+#pragma unroll
+    for (int j = 0; j < V; j++) edge_values.v[j] = edge.v[j];
+    if (edge.count > 0) add_vector<T, V>(&run, edge_values, a.scale2);
     run.join_lanes(a.scale2);
     if (t % 64 == 0) part_max[t / 64] = run.max, part_sum[t / 64] = run.sum;
     __syncthreads();
@@ -246,19 +258,17 @@ __global__ void __launch_bounds__(THREADS) custos_policy_rows(const RowArgs a) {
         for (int i = 0; i < HELD; i++) {
             const unsigned int v = t + i * THREADS;
             if (v >= vecs) break;
-            const Place<V> at(v, a.vocab);
-            store_pack<STREAM, T, V>(grad + at.first, g.of<T, V>(held[i].pack(), at.first, a.scale2));
+            store_pack<STREAM, T, V>(grad + head + v * V, g.of<T, V>(held[i].pack(), head + v * V, a.scale2));
         }
     } else {
-        for (unsigned int v = t; v < vecs; v += THREADS) {
-            const Place<V> at(v, a.vocab);
-            const Pack<T, V> y = g.of<T, V>(load_pack<false, T, V>(z + at.first), at.first, a.scale2);
-            if (at.dup == 0) {
-                store_pack<STREAM, T, V>(grad + at.first, y);
-            } else {  // (in place, the thread of the vector before may have stored its gradient over what was loaded here)
-                for (int j = at.dup; j < V; j++) grad[at.first + j] = y.v[j];
-            }
-        }
+        for (unsigned int v = t; v < vecs; v += THREADS)
+            store_pack<STREAM, T, V>(grad + head + v * V, g.of<T, V>(load_pack<false, T, V>(z + head + v * V), head + v * V, a.scale2));
+    }
+    if (edge.count > 0) {
+        const Pack<T, V> y = g.of<T, V>(edge_values, edge.first, a.scale2);
+#pragma unroll
+        for (int j = 0; j < V - 1; j++)
+            if (static_cast<unsigned int>(j) < edge.count) grad[edge.first + j] = y.v[j];
     }
 }
 
@@ -298,7 +308,7 @@ struct Kernel {
 
 template <class T, int V, int MODE, bool STREAM>
 Kernel kernel_for(unsigned int vocab) {
-    const u64 vecs = (static_cast<u64>(vocab) + V - 1) / V;
+    const u64 vecs = vocab / V;
 #define CUSTOS_ROWS(HELD, THREADS) \
     if (HELD == 0 || vecs <= static_cast<u64>(HELD) * THREADS) return {reinterpret_cast<void*>(custos_policy_rows<T, V, HELD, THREADS, MODE, STREAM>), THREADS}
     CUSTOS_ROWS(4, 64);
@@ -313,8 +323,6 @@ Kernel kernel_for(unsigned int vocab) {
 template <class T, int MODE>
 Kernel kernel_of_type(unsigned int vocab, bool stream) {
     constexpr int V = VecOf<T>::elems;
-    // (a row shorter than a vector: element by element)
-    if (vocab < static_cast<unsigned int>(V)) return {reinterpret_cast<void*>(custos_policy_rows<T, 1, 1, 64, MODE, false>), 64};
     if (MODE == kPolicy && stream) return kernel_for<T, V, kPolicy, true>(vocab);
     return kernel_for<T, V, MODE, false>(vocab);
 }
