@@ -6,6 +6,8 @@ namespace custos_hip {
 
 namespace {
 
+constexpr uint64_t kStreamBeyond = 64ull << 20;
+
 // The kernel is one of the checkpoint kinds, and the length one a launch can have.
 int32_t check_kernel(custos_hip_device* dev, const char* what, const custos_hip_kernel* kernel, Kind kind, size_t n) {
     if (!kernel) return set_error(dev, CUSTOS_HIP_ERR_INVALID_ARGUMENT, std::string(what) + ": null kernel");
@@ -23,6 +25,9 @@ uint64_t scale_bytes(size_t n) { return (n + kCheckpoint8Block - 1) / kCheckpoin
 
 int32_t launch(custos_hip_device* dev, custos_hip_kernel* kernel, const uint64_t (&ptrs)[4], int n_ptrs, size_t n, uint64_t mode,
                const Operand* ops, size_t n_ops) {
+    uint64_t moved = 0;
+    for (size_t i = 0; i < n_ops; i++) moved += ops[i].row_bytes;
+    if (moved > kStreamBeyond) mode |= 2;
     hipFunction_t fn = nullptr;
     int32_t rc = entry_point(dev, kernel, EntrySet::Single, &fn);
     if (rc != CUSTOS_HIP_OK) return rc;

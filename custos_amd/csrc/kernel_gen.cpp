@@ -651,20 +651,33 @@ std::string checkpoint8_source(const KernelSpec& k, const std::string& body) {
     s += prelude(k.dtype, k.vec_elems, k.consts.n_params);
     s += expr_fn(k, body);
     if (k.kind == Kind::UnaryGrad8) s += grad_fn(k.dtype);
+    // `mode`: bit 0 as the body says, bit 1 streams
+    auto entry = [&](const std::string& params, const std::string& args) {
+        auto body = [&](const char* stream) { return "custos_body<" + std::string(stream) + ">(" + args + ", n, mode CUSTOS_KC_ARG);\n"; };
+        return "extern \"C\" __global__ void __launch_bounds__(CUSTOS_BT)\n" + k.name + "(" + params +
+               ", const u64 n, CUSTOS_KC_ENTRY const u64 mode) {\n    if (mode & 2) " + body("true") + "    else " + body("false") + "}\n";
+    };
     s += R"(typedef vec_t vec_any __attribute__((aligned(sizeof(S))));
 typedef signed char codes_t __attribute__((ext_vector_type(CUSTOS_VEC)));
 typedef codes_t codes_any __attribute__((aligned(1)));
-// A vector that may end behind the data: `left` elements of it exist.
+// A vector that may end behind the data.  STREAM: past the caches (a template parameter: a condition around the two
+// forms of an access is merged into the ordinary one).
+template <bool STREAM>
 static __device__ __forceinline__ vec_t custos_get(const S* p, const u64 i, const u64 n) {
-    if (i + CUSTOS_VEC <= n) return *(const vec_any*)(p + i);
+    if (i + CUSTOS_VEC <= n) {
+        if (STREAM) return __builtin_nontemporal_load((const vec_any*)(p + i));
+        return *(const vec_any*)(p + i);
+    }
     vec_t v = (vec_t)(S)0;
     for (int k = 0; k < CUSTOS_VEC; k++)
         if (i + k < n) v[k] = p[i + k];
     return v;
 }
+template <bool STREAM>
 static __device__ __forceinline__ void custos_put(S* p, const u64 i, const u64 n, const vec_t v) {
     if (i + CUSTOS_VEC <= n) {
-        *(vec_any*)(p + i) = v;
+        if (STREAM) __builtin_nontemporal_store(v, (vec_any*)(p + i));
+        else *(vec_any*)(p + i) = v;
         return;
     }
     for (int k = 0; k < CUSTOS_VEC; k++)
@@ -682,12 +695,12 @@ static __device__ __forceinline__ float custos_block_max(float v) {
     return v;
 }
 )";
-        s += "extern \"C\" __global__ void __launch_bounds__(CUSTOS_BT)\n" + k.name +
-             "(const S* x, S* out, signed char* codes, float* scales, const u64 n, CUSTOS_KC_ENTRY const u64 mode) {\n";
-        s += R"(    const u64 first = ((u64)blockIdx.x * CUSTOS_UNROLL * CUSTOS_BT + threadIdx.x) * CUSTOS_VEC;
+        s += R"(template <bool STREAM>
+static __device__ __forceinline__ void custos_body(const S* x, S* out, signed char* codes, float* scales, const u64 n, const u64 mode CUSTOS_KC_PARAM) {
+    const u64 first = ((u64)blockIdx.x * CUSTOS_UNROLL * CUSTOS_BT + threadIdx.x) * CUSTOS_VEC;
     vec_t v[CUSTOS_UNROLL];
 #pragma unroll
-    for (int u = 0; u < CUSTOS_UNROLL; u++) v[u] = custos_get(x, first + (u64)u * CUSTOS_BT * CUSTOS_VEC, n);
+    for (int u = 0; u < CUSTOS_UNROLL; u++) v[u] = custos_get<STREAM>(x, first + (u64)u * CUSTOS_BT * CUSTOS_VEC, n);
 #pragma unroll
     for (int u = 0; u < CUSTOS_UNROLL; u++) {
         const u64 i = first + (u64)u * CUSTOS_BT * CUSTOS_VEC;
@@ -722,11 +735,12 @@ static __device__ __forceinline__ float custos_block_max(float v) {
             vec_t r;
 #pragma unroll
             for (int k = 0; k < CUSTOS_VEC; k++) r[k] = custos_store(custos_expr(a[k] CUSTOS_KC_ARG));
-            custos_put(out, i, n, r);
+            custos_put<STREAM>(out, i, n, r);
         }
     }
 }
 )";
+        s += entry("const S* x, S* out, signed char* codes, float* scales", "x, out, codes, scales");
         return s;
     }
     s += "static __device__ __forceinline__ C custos_restore(const signed char code, const float scale) {\n"
@@ -741,8 +755,8 @@ static __device__ __forceinline__ float custos_block_max(float v) {
 }
 )";
     const bool grad = k.kind == Kind::UnaryGrad8;
-    s += "extern \"C\" __global__ void __launch_bounds__(CUSTOS_BT)\n" + k.name + "(const signed char* codes, const float* scales, S* out, " +
-         (grad ? "const S* out_grad, " : "") + "const u64 n, CUSTOS_KC_ENTRY const u64 mode) {\n";
+    const std::string params = std::string("const signed char* codes, const float* scales, S* out") + (grad ? ", const S* out_grad" : "");
+    s += "template <bool STREAM>\nstatic __device__ __forceinline__ void custos_body(" + params + ", const u64 n, const u64 mode CUSTOS_KC_PARAM) {\n";
     s += "    const u64 first = ((u64)blockIdx.x * CUSTOS_UNROLL * CUSTOS_BT + threadIdx.x) * CUSTOS_VEC;\n"
          "    codes_t c[CUSTOS_UNROLL];\n    float scale[CUSTOS_UNROLL];\n";
     if (grad) s += "    vec_t o[CUSTOS_UNROLL], g[CUSTOS_UNROLL];\n";
@@ -750,7 +764,7 @@ static __device__ __forceinline__ float custos_block_max(float v) {
          "        const u64 i = first + (u64)u * CUSTOS_BT * CUSTOS_VEC;\n"
          "        c[u] = custos_codes(codes, i, n);\n"
          "        scale[u] = i < n ? scales[i >> 7] : 0.0f;\n";
-    if (grad) s += "        o[u] = custos_get(out_grad, i, n);\n        if (mode & 1) g[u] = custos_get(out, i, n);\n";
+    if (grad) s += "        o[u] = custos_get<STREAM>(out_grad, i, n);\n        if (mode & 1) g[u] = custos_get<STREAM>(out, i, n);\n";
     s += "    }\n#pragma unroll\n    for (int u = 0; u < CUSTOS_UNROLL; u++) {\n        vec_t r;\n";
     const std::string f = "custos_expr(custos_restore(c[u][k], scale[u]) CUSTOS_KC_ARG)";
     const std::string each = "#pragma unroll\n        for (int k = 0; k < CUSTOS_VEC; k++) r[k] = custos_store(";
@@ -759,7 +773,8 @@ static __device__ __forceinline__ float custos_block_max(float v) {
     else
         s += "        if (mode & 1) {\n" + each + "custos_grad(custos_load(g[u][k]), custos_load(o[u][k]), " + f + "));\n        } else {\n" +
              each + "custos_load(o[u][k]) * " + f + ");\n        }\n";
-    s += "        custos_put(out, first + (u64)u * CUSTOS_BT * CUSTOS_VEC, n, r);\n    }\n    (void)mode;\n}\n";
+    s += "        custos_put<STREAM>(out, first + (u64)u * CUSTOS_BT * CUSTOS_VEC, n, r);\n    }\n    (void)mode;\n}\n";
+    s += entry(params, grad ? "codes, scales, out, out_grad" : "codes, scales, out");
     return s;
 }
 

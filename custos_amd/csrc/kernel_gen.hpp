@@ -28,7 +28,7 @@ enum class Kind : int32_t {
 // The kinds that work on 8-bit checkpoints (custos_hip_checkpoint8_*): one marker, one entry point.
 inline bool checkpoint8_kind(Kind kind) { return kind == Kind::Save8 || kind == Kind::Restore8 || kind == Kind::UnaryGrad8; }
 constexpr int kCheckpoint8Block = 128;    // elements that share a scale
-constexpr int kCheckpoint8Threads = 256;  // per workgroup
+constexpr int kCheckpoint8Threads = 64;   // per workgroup
 constexpr int kCheckpoint8Unroll = 2;     // 16-byte vectors per thread
 
 struct Tuning {

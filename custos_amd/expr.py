@@ -11,6 +11,9 @@ its GPU backends; that string is what the C ABI compiles.
 """
 from __future__ import annotations
 
+import functools
+import math
+
 import numpy as np
 
 _BINARY_INFIX = {"add": "+", "sub": "-", "mul": "*", "div": "/", "geq": ">=", "leq": "<=", "eq": "=="}
@@ -107,10 +110,18 @@ class Const(Expr):
 def format_float(v: float, dtype: str = "f32") -> str:
     """Shortest text that round-trips in the element type, with Rust's spelling
     of whole numbers ("2.0"), infinities ("inf") and NaN ("NaN")."""
-    if np.isnan(v):
+    if v != v:
         return "NaN"
-    if np.isinf(v):
+    if v in (math.inf, -math.inf):
         return "inf" if v > 0 else "-inf"
+    # (the sign apart: 0.0 and -0.0 are equal keys)
+    return _format_finite(v, math.copysign(1.0, v), dtype)
+
+
+@functools.lru_cache(maxsize=4096)
+def _format_finite(v: float, sign: float, dtype: str) -> str:
+    """The text of a value does not change, and numpy takes some microseconds to find it: a closure is printed
+    again for every launch."""
     if dtype == "f64":
         s = repr(float(v))
     else:
