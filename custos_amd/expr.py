@@ -68,24 +68,26 @@ class Expr:
         raise NotImplementedError
 
 
+# how every node prints, over the texts of its operands
+_TEXT = {op: f"(%s {sign} %s)" for op, sign in _BINARY_INFIX.items()}
+_TEXT.update({op: f"{name}(%s, %s)" for op, name in _BINARY_CALL.items()})
+_TEXT.update({op: f"{name}(%s)" for op, name in _UNARY_CALL.items()})
+_TEXT.update({"neg": "-(%s)", "identity": "%s"})
+
+
 class Node(Expr):
     def __init__(self, op, *args):
         self.op = op
         self.args = args
 
     def to_cl_source(self, dtype: str = "f32") -> str:
-        a = [x.to_cl_source(dtype) for x in self.args]
-        if self.op in _BINARY_INFIX:
-            return f"({a[0]} {_BINARY_INFIX[self.op]} {a[1]})"
-        if self.op in _BINARY_CALL:
-            return f"{_BINARY_CALL[self.op]}({a[0]}, {a[1]})"
-        if self.op in _UNARY_CALL:
-            return f"{_UNARY_CALL[self.op]}({a[0]})"
-        if self.op == "neg":
-            return f"-({a[0]})"
-        if self.op == "identity":
-            return a[0]
-        raise ValueError(self.op)
+        text = _TEXT.get(self.op)
+        if text is None:
+            raise ValueError(self.op)
+        args = self.args
+        if len(args) == 2:
+            return text % (args[0].to_cl_source(dtype), args[1].to_cl_source(dtype))
+        return text % args[0].to_cl_source(dtype)
 
 
 class Const(Expr):
@@ -98,6 +100,8 @@ class Const(Expr):
 
     def to_cl_source(self, dtype: str = "f32") -> str:
         v = self.value
+        if type(v) is float:  # (by far the most)
+            return format_float(v, dtype)
         if isinstance(v, str):
             return v
         if isinstance(v, (bool, np.bool_)):
