@@ -13,12 +13,13 @@ int32_t check_kernel(custos_hip_device* dev, const char* what, const custos_hip_
     if (!kernel) return set_error(dev, CUSTOS_HIP_ERR_INVALID_ARGUMENT, std::string(what) + ": null kernel");
     if (kernel->spec.kind != kind)
         return set_error(dev, CUSTOS_HIP_ERR_KIND_MISMATCH, std::string(what) + ": the kernel was compiled as another kind");
-    if (n > (1ull << 40)) return set_error(dev, CUSTOS_HIP_ERR_TOO_LARGE, std::string(what) + ": more than 2^40 elements");
+    // (of one launch, which has fewer than 2^32 threads)
+    if (n > (1ull << 34)) return set_error(dev, CUSTOS_HIP_ERR_TOO_LARGE, std::string(what) + ": more than 2^34 elements");
     return CUSTOS_HIP_OK;
 }
 
-Operand flat(const char* name, uint64_t ptr, uint64_t bytes, bool written, size_t element) {
-    return {name, ptr, 1, bytes, 0, written, element};
+Operand flat(const char* name, uint64_t ptr, uint64_t bytes, bool written, size_t element, bool in_place = false) {
+    return {name, ptr, 1, bytes, 0, written, element, in_place};
 }
 
 uint64_t scale_bytes(size_t n) { return (n + kCheckpoint8Block - 1) / kCheckpoint8Block * sizeof(float); }
@@ -72,10 +73,10 @@ int32_t custos_hip_checkpoint8_save(custos_hip_device* dev, custos_hip_kernel* k
     REQUIRE_DEV(dev);
     if (n == 0) return CUSTOS_HIP_OK;
     const size_t es = dtype_size(kernel->spec.dtype);
-    Operand ops[4] = {flat("x", x, n * es, false, es), flat("codes", codes, n, true, 1), flat("scales", scales, scale_bytes(n), true, 4)};
+    Operand ops[4] = {flat("x", x, n * es, false, es, true), flat("codes", codes, n, true, 1), flat("scales", scales, scale_bytes(n), true, 4)};
     size_t n_ops = 3;
-    if (out) ops[n_ops++] = flat("out", out, n * es, true, es);
-    rc = check_operands(dev, what, ops, n_ops, /*may_alias=*/true);
+    if (out) ops[n_ops++] = flat("out", out, n * es, true, es, true);
+    rc = check_operands(dev, what, ops, n_ops);
     if (rc != CUSTOS_HIP_OK) return rc;
     return launch(dev, kernel, {x, out, codes, scales}, 4, n, out ? 1 : 0, ops, n_ops);
 }
@@ -90,7 +91,7 @@ int32_t custos_hip_checkpoint8_restore(custos_hip_device* dev, custos_hip_kernel
     const size_t es = dtype_size(kernel->spec.dtype);
     const Operand ops[3] = {flat("codes", codes, n, false, 1), flat("scales", scales, scale_bytes(n), false, 4),
                             flat("out", out, n * es, true, es)};
-    rc = check_operands(dev, what, ops, 3, /*may_alias=*/false);
+    rc = check_operands(dev, what, ops, 3);
     if (rc != CUSTOS_HIP_OK) return rc;
     return launch(dev, kernel, {codes, scales, out, 0}, 3, n, 0, ops, 3);
 }
@@ -106,8 +107,8 @@ int32_t custos_hip_add_unary_grad8(custos_hip_device* dev, custos_hip_kernel* ke
     const bool overwrite = (flags & CUSTOS_HIP_GRAD_OVERWRITE) != 0;
     const size_t es = dtype_size(kernel->spec.dtype);
     const Operand ops[4] = {flat("codes", codes, n, false, 1), flat("scales", scales, scale_bytes(n), false, 4),
-                            flat("lhs_grad", lhs_grad, n * es, true, es), flat("out_grad", out_grad, n * es, false, es)};
-    rc = check_operands(dev, what, ops, 4, /*may_alias=*/overwrite);
+                            flat("lhs_grad", lhs_grad, n * es, true, es, overwrite), flat("out_grad", out_grad, n * es, false, es, true)};
+    rc = check_operands(dev, what, ops, 4);
     if (rc != CUSTOS_HIP_OK) return rc;
     return launch(dev, kernel, {codes, scales, lhs_grad, out_grad}, 4, n, overwrite ? 0 : 1, ops, 4);
 }

@@ -14,10 +14,11 @@
 //
 // Statistics are held in f32 and never as a difference of large sums: a mean, and the sum of squared
 // distances from it (merged as count, mean and that sum), in f64 where the parts of a group are joined.
-// h and z are each rounded as written (no fused multiply-add), so that the branch of an activation at
+// In the gradient h and z are each rounded as written (no fused multiply-add), so that the branch of an activation at
 // z = 0 is the one that 32-bit arithmetic takes anywhere else.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "op_device.hpp"
 #include "runtime.hpp"
@@ -27,14 +28,14 @@ namespace custos_hip {
 namespace {
 
 constexpr int kBlock = 256;      // threads of the kernels that stream
-constexpr int kMaxTileGroups = 64;     // groups per tile of the kernels that hold a tile in registers
+constexpr unsigned int kMaxTileGroups = 64;     // groups per tile of the kernels that hold a tile in registers
 constexpr int kMaxStreamGroups = 128;  // groups per tile of the kernels that stream
 
 enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 
 // Division of 32-bit numbers by one the host knows.
 struct Divisor {
-    unsigned int by = 1, magic = 0;  // floor(2^32 / by); by == 1: 0, and the correction below gives the answer
+    unsigned int by, magic;  // floor(2^32 / by); by == 1: 0, and the correction below gives the answer
     __device__ __forceinline__ unsigned int divide(unsigned int n) const {
         if (by == 1) return n;
         unsigned int q = __umulhi(n, magic);  // (at most one too small)
@@ -44,8 +45,8 @@ struct Divisor {
 // How the rows of a sample are dealt out to workgroups: `rounds` rounds of `step` rows each, to the first `longer` of
 // them one more.
 struct Splits {
-    unsigned int count = 1, longer = 0;
-    u64 rounds = 0;
+    unsigned int count, longer;
+    u64 rounds;
     Divisor by_count;
 };
 
@@ -62,7 +63,7 @@ struct GroupNormArgs {
     // a tile in registers).  Forward: [samples][parts][groups] pairs of a mean and a sum of squared
     // distances.  Backward: the same of the sums of dz * gamma and of dz * gamma * h, and `channel_parts`.
     float* group_parts;
-    float* channel_parts;     // [samples][parts][2][channels]: sums of dz and of dz * h
+    float* channel_parts;     // [channel_rows][2][channels]: sums of dz and of dz * h
     float* gamma_grad;
     float* beta_grad;
     u64 positions;
@@ -78,6 +79,7 @@ struct GroupNormArgs {
     unsigned int part_step;        // the first pass's
     unsigned int last_part, missing_rows;  // the part with the last round of rows, and how many that is short of `step`
     unsigned int blocks;           // workgroups that work on values; what follows them adds up gamma_grad and beta_grad
+    unsigned int channel_rows;     // of channel_parts: a part each, or the samples that one workgroup takes
     unsigned int per_group_magic;  // ceil(2^32 / per_group), for divisions of numbers below 2^16
     int param_f32, accumulate;
     float eps;
@@ -88,13 +90,7 @@ __device__ __forceinline__ unsigned int group_of(unsigned int e, unsigned int ma
     return magic ? __umulhi(e, magic) : e;
 }
 
-template <class T>
-__device__ __forceinline__ float param(const void* p, int f32, unsigned int i, float none) {
-    if (!p) return none;
-    return f32 ? static_cast<const float*>(p)[i] : to_f32(static_cast<const T*>(p)[i]);
-}
-
-// V of them, with one branch and wide loads.
+// gamma or beta of V neighbouring channels, with one branch and wide loads.
 template <class T, int V>
 __device__ __forceinline__ void params(const void* p, int f32, unsigned int first, float none, float (&out)[V]) {
     if (!p) {
@@ -267,7 +263,7 @@ __device__ __forceinline__ void merge_groups(const GroupNormArgs& a, const float
 // Sum over the workgroup, in every thread.
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float* wave_sums) {
-    v = lanes_sum<64>(v);
+    v = lanes_sum(v);
     __syncthreads();
     if (threadIdx.x % 64 == 0) wave_sums[threadIdx.x / 64] = v;
     __syncthreads();
@@ -348,7 +344,7 @@ __global__ void __launch_bounds__(THREADS) custos_group_norm_tile(const GroupNor
         for (int j = 0; j < V; j++) mean[j] = m2[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
-            if (static_cast<unsigned int>(i) >= rounds) break;
+            if (static_cast<unsigned int>(i) >= rounds) continue;
             const Pack<T, V> p = held[i].pack();
 #pragma unroll
             for (int j = 0; j < V; j++) mean[j] += to_f32(p.v[j]);
@@ -359,7 +355,7 @@ __global__ void __launch_bounds__(THREADS) custos_group_norm_tile(const GroupNor
         for (int j = 0; j < V; j++) mean[j] *= inverse;
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
-            if (static_cast<unsigned int>(i) >= rounds) break;
+            if (static_cast<unsigned int>(i) >= rounds) continue;
             const Pack<T, V> p = held[i].pack();
 #pragma unroll
             for (int j = 0; j < V; j++) {
@@ -393,7 +389,7 @@ __global__ void __launch_bounds__(THREADS) custos_group_norm_tile(const GroupNor
     T* out = static_cast<T*>(a.out) + (static_cast<u64>(n) * a.positions + r0) * a.out_pitch + c0 + c.first;
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-        if (static_cast<unsigned int>(i) >= rounds) break;
+        if (static_cast<unsigned int>(i) >= rounds) continue;
         const Pack<T, V> p = held[i].pack();
         Pack<T, V> y;
 #pragma unroll
@@ -659,11 +655,11 @@ __device__ __forceinline__ void store_grad(const GroupNormArgs& a, T* p, float (
 }
 
 // From a thread's sums s1 (dz) and s2 (dz * h) of its column: those of the channels over the rows of the workgroup,
-// to `channel`, and from there, times gamma, those of the groups, to sums_of.
+// to `channel` (`adds`: to what the same thread put there), and from there, times gamma, those of the groups, to sums_of.
 template <int V, int THREADS>
 __device__ __forceinline__ void channel_and_group_sums(const GroupNormArgs& a, const Column& c, unsigned int r0, unsigned int step,
                                                        const float (&s1)[V], const float (&s2)[V], const float (&gamma_of)[V], float2* table, float* gammas,
-                                                       float* channel, float2* sums_of) {
+                                                       float* channel, bool adds, float2* sums_of) {
     const unsigned int t = threadIdx.x;
     if (r0 == 0) {
 #pragma unroll
@@ -691,8 +687,8 @@ __device__ __forceinline__ void channel_and_group_sums(const GroupNormArgs& a, c
             }
         for (unsigned int half = lanes / 2; half > 0; half /= 2) x += __shfl_xor(x, half, 64), y += __shfl_xor(y, half, 64);
         if (ch < c.width && t % lanes == 0) {
-            channel[ch] = x;
-            channel[a.channels + ch] = y;
+            channel[ch] = adds ? channel[ch] + x : x;
+            channel[a.channels + ch] = adds ? channel[a.channels + ch] + y : y;
             const float gamma = gammas[ch];
             table[ch] = make_float2(x * gamma, y * gamma);  // (only these lanes read column ch, and they have)
         }
@@ -717,99 +713,103 @@ __device__ __forceinline__ void channel_and_group_sums(const GroupNormArgs& a, c
 
 // gamma_grad and beta_grad of 16 channels, by one workgroup: the sums of all parts of all samples, in a fixed order.
 constexpr int kParamChannels = 16;
-__device__ __forceinline__ void param_grads(const GroupNormArgs& a, unsigned int block, float* sums) {
+__device__ __forceinline__ void param_grads(const GroupNormArgs& a, unsigned int block, double* sums) {
     const unsigned int t = threadIdx.x, which = t / kParamChannels % 2, lane = t / (2 * kParamChannels);
     constexpr unsigned int kLanes = kBlock / (2 * kParamChannels);
     const unsigned int ch = block * kParamChannels + t % kParamChannels;
-    float s = 0.0f;
+    double s = 0.0;
     if (ch < a.channels)
 #pragma unroll 4
-        for (unsigned int row = lane; row < a.samples * a.parts.count; row += kLanes)
+        for (unsigned int row = lane; row < a.channel_rows; row += kLanes)
             s += a.channel_parts[(static_cast<u64>(row) * 2 + which) * a.channels + ch];
     sums[t] = s;
     __syncthreads();
     if (lane > 0 || ch >= a.channels) return;
     for (unsigned int l = 1; l < kLanes; l++) s += sums[l * 2 * kParamChannels + t];
     float* out = which ? a.gamma_grad : a.beta_grad;
-    if (out) out[ch] = a.accumulate ? out[ch] + s : s;
+    if (out) out[ch] = static_cast<float>(a.accumulate ? out[ch] + s : s);
 }
 
 __global__ void __launch_bounds__(kBlock) custos_group_norm_param_grads(const GroupNormArgs a) {
-    __shared__ float sums[kBlock];
+    __shared__ double sums[kBlock];
     param_grads(a, blockIdx.x, sums);
 }
 
-// A tile in registers: x and out_grad read once.
+// A tile in registers: x and out_grad read once.  With more samples than the chip holds workgroups for, each takes
+// several, `channel_rows` apart, so that the work area and what is added up behind stay small.  (Nothing in shared
+// memory is written again before a barrier that follows its last read.)
 template <class T, int V, int HELD, int THREADS, bool SAVED, int ACT>
 __global__ void __launch_bounds__(THREADS) custos_group_norm_grad_tile(const GroupNormArgs a) {
     __shared__ float2 table[THREADS * V];
     __shared__ float gammas[THREADS * V];
     __shared__ float2 sums_of[kMaxTileGroups];
     const unsigned int t = threadIdx.x;
-    const unsigned int index = by_xcd(blockIdx.x, gridDim.x), n = a.by_tiles.divide(index), tile = index - n * a.tiles;
+    const unsigned int index = by_xcd(blockIdx.x, gridDim.x), sample0 = a.by_tiles.divide(index), tile = index - sample0 * a.tiles;
     const unsigned int vecs = a.vecs, step = a.step;
     const unsigned int r0 = group_of(t, a.vecs_magic);
     const Column c = column_of<V>(a, t - r0 * vecs);
     const bool active = r0 < step;
     const unsigned int c0 = tile * a.tile_groups * a.per_group;
-    const u64 row0 = static_cast<u64>(n) * a.positions;
-    const T* out_grad = static_cast<const T*>(a.out_grad) + row0 * a.grad_pitch + c0 + c.first;
-    Source<T, V, SAVED> held[HELD];
-    Bits<T, V> grad[HELD];
-#pragma unroll
-    for (int i = 0; i < HELD; i++) {
-        const u64 p = r0 + static_cast<u64>(i) * step;
-        if (active && p < a.positions) {
-            held[i].load(a, row0 + p, c0 + c.first);
-            grad[i].load(out_grad + p * a.grad_pitch);
-        } else {
-            held[i].zero();
-            grad[i].zero();
-        }
-    }
-    ChannelParams<T, V> k;
-    k.load(a, n, tile, c);
-    float s1[V], s2[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.0f;
-    {
-#pragma unroll
-        for (int i = 0; i < HELD; i++) {
-            if (r0 + static_cast<u64>(i) * step >= a.positions) break;
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                float h;
-                const float dz = dz_of<ACT>(k, j, held[i].value(j), to_f32(grad[i].pack().v[j]), &h);
-                s1[j] += dz;
-                s2[j] = __builtin_fmaf(dz, h, s2[j]);
-            }
-            held[i].forget_values();
-            grad[i].forget_values();
-        }
-    }
-    channel_and_group_sums<V, THREADS>(a, c, r0, step, s1, s2, k.gamma, table, gammas, a.channel_parts + static_cast<u64>(n) * 2 * a.channels + c0, sums_of);
-    if (!a.out || !active) return;
-    const float count = static_cast<float>(a.positions) * static_cast<float>(a.per_group);
-    const GradientOf<T, V> gradient(k, [&](int j, float* dh, float* dhh) {
-        const unsigned int g = group_of(c.first + j, a.per_group_magic);
-        const float2 both = sums_of[g];
-        *dh = both.x / count;
-        *dhh = both.y / count;
-    });
-    T* out = static_cast<T*>(a.out) + row0 * a.out_pitch + c0 + c.first;
-    {
+    for (unsigned int n = sample0; n < a.samples; n += a.channel_rows) {
+        const u64 row0 = static_cast<u64>(n) * a.positions;
+        const T* out_grad = static_cast<const T*>(a.out_grad) + row0 * a.grad_pitch + c0 + c.first;
+        Source<T, V, SAVED> held[HELD];
+        Bits<T, V> grad[HELD];
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
             const u64 p = r0 + static_cast<u64>(i) * step;
-            if (p >= a.positions) break;
-            float g[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                float h;
-                const float dz = dz_of<ACT>(k, j, held[i].value(j), to_f32(grad[i].pack().v[j]), &h);
-                g[j] = gradient.of(j, dz, h);
+            if (active && p < a.positions) {
+                held[i].load(a, row0 + p, c0 + c.first);
+                grad[i].load(out_grad + p * a.grad_pitch);
+            } else {
+                held[i].zero();
+                grad[i].zero();
             }
-            store_grad<false, T, V>(a, out + p * a.out_pitch, g);
+        }
+        ChannelParams<T, V> k;
+        k.load(a, n, tile, c);
+        float s1[V], s2[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.0f;
+        {
+#pragma unroll
+            for (int i = 0; i < HELD; i++) {
+                if (r0 + static_cast<u64>(i) * step >= a.positions) break;
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    float h;
+                    const float dz = dz_of<ACT>(k, j, held[i].value(j), to_f32(grad[i].pack().v[j]), &h);
+                    s1[j] += dz;
+                    s2[j] = __builtin_fmaf(dz, h, s2[j]);
+                }
+                held[i].forget_values();
+                grad[i].forget_values();
+            }
+        }
+        channel_and_group_sums<V, THREADS>(a, c, r0, step, s1, s2, k.gamma, table, gammas, a.channel_parts + static_cast<u64>(sample0) * 2 * a.channels + c0, n != sample0, sums_of);
+        if (!a.out || !active) continue;
+        const float count = static_cast<float>(a.positions) * static_cast<float>(a.per_group);
+        const GradientOf<T, V> gradient(k, [&](int j, float* dh, float* dhh) {
+            const unsigned int g = group_of(c.first + j, a.per_group_magic);
+            const float2 both = sums_of[g];
+            *dh = both.x / count;
+            *dhh = both.y / count;
+        });
+        T* out = static_cast<T*>(a.out) + row0 * a.out_pitch + c0 + c.first;
+        {
+#pragma unroll
+            for (int i = 0; i < HELD; i++) {
+                const u64 p = r0 + static_cast<u64>(i) * step;
+                if (p >= a.positions) break;
+                float g[V];
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    float h;
+                    const float dz = dz_of<ACT>(k, j, held[i].value(j), to_f32(grad[i].pack().v[j]), &h);
+                    g[j] = gradient.of(j, dz, h);
+                }
+                store_grad<false, T, V>(a, out + p * a.out_pitch, g);
+            }
         }
     }
 }
@@ -890,14 +890,14 @@ __global__ void __launch_bounds__(kBlock) custos_group_norm_grad_parts(const Gro
         if (t == 0) group[0] = dh, group[1] = dhh;
         return;
     }
-    channel_and_group_sums<V, kBlock>(a, c, w.r0, w.step, s1, s2, k.gamma, table, gammas, channel, sums_of);
+    channel_and_group_sums<V, kBlock>(a, c, w.r0, w.step, s1, s2, k.gamma, table, gammas, channel, false, sums_of);
     for (unsigned int g = t; g < a.tile_groups; g += kBlock) reinterpret_cast<float2*>(group)[g] = sums_of[g];
 }
 
 // x_grad, and by the workgroups behind the first `blocks` gamma_grad and beta_grad.
 template <class T, int V, bool SAVED, int ACT, bool STREAM>
 __global__ void __launch_bounds__(kBlock) custos_group_norm_grad_values(const GroupNormArgs a) {
-    __shared__ float sums[kBlock];
+    __shared__ double sums[kBlock];
     if (blockIdx.x >= a.blocks) {
         param_grads(a, blockIdx.x - a.blocks, sums);
         return;
@@ -937,6 +937,9 @@ __global__ void __launch_bounds__(kBlock) custos_group_norm_grad_values(const Gr
 // What the plans below go by, in microseconds measured on MI355X (kernels alone):
 // - Rows of a tile in registers are at least 32 bytes: twice the workgroups of 64-byte rows, 8x1024x640 bf16 in
 //   12.8 against 14.6 (41 with 128 bytes); the tiles that share a cache line run on one XCD.
+//   Wider ones while 256 threads hold them with four vectors each and 1024 tiles are left: every workgroup waits for
+//   the same few loads and barriers, however little it moves.  512x64x640 bf16 in 26 forward and 71 backward, against 56
+//   and 150 with rows of 32 bytes; 64x64x1280 in 11 and 20 against 15 and 28.
 // - Rows of a tile that is streamed are at least 128 bytes: the second pass of the gradient over 4x4096x320 bf16
 //   takes 10.9, with 256 bytes 12.2, with 64 bytes 15.2; the first pass 11.8, 11.4, 13.7.  Where the data does not
 //   stay in the caches, 256 bytes: gradient over 8x16384x512 bf16 from codes 49 + 57, with 128 bytes 50 + 79, with
@@ -947,6 +950,10 @@ __global__ void __launch_bounds__(kBlock) custos_group_norm_grad_values(const Gr
 //   first pass read and leave dirty lines to be written back during the next pass.  16x16384x512 f16: first pass
 //   55 and second 88 that way, 85 and 102 through the caches.
 constexpr unsigned int kTileRow = 32, kStreamRow = 128;
+// - Tiles in registers, backward: beyond 2^21 threads, four times what the chip holds at once, a workgroup takes
+//   several samples.
+constexpr u64 kTilesEnough = 1024;
+constexpr u64 kThreadsTogether = 1ull << 21;
 constexpr u64 kTileAlone = 16384, kTilesTogether = 128, kStreamBeyond = 64ull << 20;
 
 struct Plan {
@@ -955,7 +962,9 @@ struct Plan {
     int threads = kBlock;
     int held = 0;
     bool stream = false;  // the second pass loads and stores past the caches
-    GroupNormArgs a{};
+    GroupNormArgs a;
+    // (padding included: recordings compare the arguments of their launches byte by byte)
+    Plan() { std::memset(&a, 0, sizeof a); }
 };
 
 Divisor divisor(unsigned int by) { return {by, by == 1 ? 0u : static_cast<unsigned int>(0x100000000ull / by)}; }
@@ -973,12 +982,18 @@ unsigned int tile_at_least(unsigned int groups, unsigned int per_group, unsigned
         }
     return best;
 }
-// (threads, vectors held) of the kernels that hold a tile in registers, smallest first.
+// (threads, vectors held) of the kernels that hold a tile in registers, smallest first, and the most bytes moved they
+// are used for: one reading of x in rows of 32 bytes against two readings in wide ones, the second of which finds x
+// in the caches.  Forward, 1024 x 8: 8x4096x512 bf16 (64 MiB) in 22 against 27 streamed, 16x4096x512 in 49 against 41;
+// 1024 x 16: 4x4096x640 bf16 (40 MiB) in 23 against 26, 4x4096x512 f32 in 20 against 24, but 4x7000x512 bf16 in 29
+// against 26.  Backward, 512 x 4: 4x256x1280 bf16 (7.5 MiB) in 12 against 20, 8x256x1280 in 13 against 20, 8x1024x320
+// in 19 both ways, 16x512x1024 (48 MiB) in 27 against 24; 1024 threads leave that kernel too few registers.
 struct Held {
     int threads, held;
+    u64 most;
 };
-constexpr Held kForwardHeld[] = {{256, 4}, {256, 8}, {1024, 4}, {1024, 8}, {1024, 16}};
-constexpr Held kBackwardHeld[] = {{256, 4}, {1024, 4}};
+constexpr Held kForwardHeld[] = {{256, 4, ~0ull}, {256, 8, ~0ull}, {1024, 4, ~0ull}, {1024, 8, kStreamBeyond}, {1024, 16, kStreamBeyond}};
+constexpr Held kBackwardHeld[] = {{256, 4, ~0ull}, {512, 4, 32ull << 20}};
 
 // `accumulates`: the results are added to what is there, so no channel may be stored by two threads.
 template <size_t N>
@@ -1012,12 +1027,17 @@ void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool
     };
     // in registers, if a tile of whole groups of at least 64 bytes a row fits
     {
-        const unsigned int k = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>(kTileRow / elem), kMaxTileGroups);
+        unsigned int k = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>(kTileRow / elem), kMaxTileGroups);
+        for (unsigned int wider = k + 1; wider <= std::min(a.groups, kMaxTileGroups); wider++) {
+            const u64 row = (static_cast<u64>(wider) * a.per_group + full - 1) / full;
+            if (row > kBlock || a.positions > 4 * (kBlock / row) || static_cast<u64>(a.samples) * (a.groups / wider) < kTilesEnough) break;
+            if (a.groups % wider == 0) k = wider;
+        }
         const u64 width = static_cast<u64>(k) * a.per_group;
         const unsigned int vec = width < full || (accumulates && width % full != 0) ? 1 : full;
         const u64 vecs = (width + vec - 1) / vec;
         for (const Held& h : choices) {
-            if (vecs > static_cast<u64>(h.threads)) continue;
+            if (vecs > static_cast<u64>(h.threads) || moved > h.most) continue;
             const u64 step = static_cast<u64>(h.threads) / vecs;
             if ((a.positions + step - 1) / step > static_cast<u64>(h.held)) continue;
             if (a.positions * width > kTileAlone && static_cast<u64>(a.samples) * (a.groups / k) < kTilesTogether) continue;
@@ -1074,17 +1094,14 @@ int32_t check_desc(custos_hip_device* dev, const char* what, const custos_hip_gr
     if (d->activation < 0 || d->activation > CUSTOS_HIP_ACT_GELU) return bad("unknown activation");
     if (d->flags & ~CUSTOS_HIP_GRAD_OVERWRITE) return bad("unknown flag");
     if (d->channels == 0 || d->groups == 0 || d->channels % d->groups != 0) return bad("the channels divide into the groups");
-    if (!(d->eps > 0) || !std::isfinite(d->eps)) return bad("eps is positive");
+    // (as the kernels hold it: a group of equal values divides by its root)
+    if (!(d->eps > 0) || !std::isnormal(static_cast<float>(d->eps))) return bad("eps is positive, and a normal number in f32");
     if (d->channels >= (1ull << 30) || d->samples >= (1ull << 31) || d->positions >= (1ull << 40) ||
         static_cast<double>(d->samples) * static_cast<double>(d->positions) * static_cast<double>(d->channels) > 1e15)
         return set_error(dev, CUSTOS_HIP_ERR_TOO_LARGE, std::string(what) + ": the sizes are beyond any memory");
     return CUSTOS_HIP_OK;
 }
 
-int32_t check_grid(custos_hip_device* dev, const char* what, u64 blocks) {
-    if (blocks >= (1ull << 31)) return set_error(dev, CUSTOS_HIP_ERR_TOO_LARGE, std::string(what) + ": more than 2^31 workgroups");
-    return CUSTOS_HIP_OK;
-}
 
 template <class K>
 void* handle(K* kernel) {
@@ -1127,8 +1144,8 @@ Kernel backward_tile(const Plan& p) {
     constexpr int V = VecOf<T>::elems;
     const char* name = "custos_group_norm_grad_tile";
     const bool wide = p.vec > 1;
-    if (p.threads == 1024)
-        return {wide ? handle(custos_group_norm_grad_tile<T, V, 4, 1024, SAVED, ACT>) : handle(custos_group_norm_grad_tile<T, 1, 4, 1024, SAVED, ACT>), name};
+    if (p.threads == 512)
+        return {wide ? handle(custos_group_norm_grad_tile<T, V, 4, 512, SAVED, ACT>) : handle(custos_group_norm_grad_tile<T, 1, 4, 512, SAVED, ACT>), name};
     return {wide ? handle(custos_group_norm_grad_tile<T, V, 4, 256, SAVED, ACT>) : handle(custos_group_norm_grad_tile<T, 1, 4, 256, SAVED, ACT>), name};
 }
 template <class T, int ACT, bool SAVED>
@@ -1195,15 +1212,14 @@ int32_t custos_hip_group_norm(custos_hip_device* dev, const custos_hip_group_nor
     }
     const size_t es = elem_size(desc->dtype), ps = elem_size(desc->param_dtype);
     const u64 rows = desc->samples * desc->positions;
-    Operand ops[5] = {{"out", out, rows, desc->channels * es, out_pitch * es, true, es},
+    Operand ops[5] = {{"out", out, rows, desc->channels * es, out_pitch * es, true, es, true},
                       {"stats", stats, 1, desc->samples * desc->groups * 8, 0, true, 4},
-                      {"x", x, rows, desc->channels * es, x_pitch * es, false, es}};
+                      {"x", x, rows, desc->channels * es, x_pitch * es, false, es, true}};
     size_t n = 3;
     if (gamma) ops[n++] = {"gamma", gamma, 1, desc->channels * ps, 0, false, ps};
     if (beta) ops[n++] = {"beta", beta, 1, desc->channels * ps, 0, false, ps};
-    rc = check_operands(dev, "group norm", ops, n, /*may_alias=*/true);
+    rc = check_operands(dev, "group norm", ops, n);
     if (rc != CUSTOS_HIP_OK) return rc;
-    REQUIRE_DEV(dev);
 
     Plan plan;
     make_plan(*desc, es, 2 * rows * desc->channels * es, /*accumulates=*/false, kForwardHeld, &plan);
@@ -1219,8 +1235,9 @@ int32_t custos_hip_group_norm(custos_hip_device* dev, const custos_hip_group_nor
     Access acc[6];
     for (size_t i = 0; i < n; i++) acc[i] = ops[i].access();
     const u64 parts = static_cast<u64>(a.samples) * a.parts.count, blocks = parts * a.tiles;
-    rc = check_grid(dev, "group norm", std::max<u64>(blocks, static_cast<u64>(a.samples) * a.tiles * a.values.count));
+    rc = check_grid(dev, "group norm", plan.in_registers ? blocks : static_cast<u64>(a.samples) * a.tiles * std::max(a.parts.count, a.values.count), plan.threads);
     if (rc != CUSTOS_HIP_OK) return rc;
+    REQUIRE_DEV(dev);
     if (plan.in_registers)
         return launch(dev, kernel_for(*desc, [&](auto t, auto act) { return forward_tile<decltype(t), act.value>(plan); }), blocks, plan.threads, a, acc, n);
 
@@ -1260,26 +1277,28 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device* dev, const custos_hip_
     }
     Operand ops[9];
     size_t n = 0;
-    if (x_grad) ops[n++] = {"x_grad", x_grad, rows, desc->channels * es, x_grad_pitch * es, true, es};
+    if (x_grad) ops[n++] = {"x_grad", x_grad, rows, desc->channels * es, x_grad_pitch * es, true, es, overwrite};
     const size_t values_written = n;
     if (gamma_grad) ops[n++] = {"gamma_grad", gamma_grad, 1, desc->channels * 4, 0, true, 4};
     if (beta_grad) ops[n++] = {"beta_grad", beta_grad, 1, desc->channels * 4, 0, true, 4};
     const size_t first_read = n;
-    ops[n++] = {"out_grad", out_grad, rows, desc->channels * es, out_grad_pitch * es, false, es};
+    ops[n++] = {"out_grad", out_grad, rows, desc->channels * es, out_grad_pitch * es, false, es, true};
     if (saved) {
         ops[n++] = {"codes", codes, 1, total, 0, false, 1};
         ops[n++] = {"scales", scales, 1, (total + 127) / 128 * 4, 0, false, 4};
     } else {
-        ops[n++] = {"x", x, rows, desc->channels * es, x_pitch * es, false, es};
+        ops[n++] = {"x", x, rows, desc->channels * es, x_pitch * es, false, es, true};
     }
     ops[n++] = {"stats", stats, 1, desc->samples * desc->groups * 8, 0, false, 4};
     if (gamma) ops[n++] = {"gamma", gamma, 1, desc->channels * ps, 0, false, ps};
     if (beta) ops[n++] = {"beta", beta, 1, desc->channels * ps, 0, false, ps};
     static_assert(sizeof ops / sizeof ops[0] >= 9, "three written, six read");
-    rc = check_operands(dev, what, ops, n, /*may_alias=*/overwrite);
+    rc = check_operands(dev, what, ops, n);
     if (rc != CUSTOS_HIP_OK) return rc;
-    REQUIRE_DEV(dev);
-    if (first_read == 0) return CUSTOS_HIP_OK;  // no gradient is wanted
+    if (first_read == 0) {  // no gradient is wanted
+        REQUIRE_DEV(dev);
+        return CUSTOS_HIP_OK;
+    }
 
     Plan plan;
     make_plan(*desc, es, total * (saved ? 2 * es + 1 : 3 * es),
@@ -1298,10 +1317,17 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device* dev, const custos_hip_
     a.out_pitch = x_grad_pitch;
     a.param_f32 = desc->param_dtype == CUSTOS_HIP_F32;
     a.accumulate = !overwrite;
-    const u64 parts = static_cast<u64>(a.samples) * a.parts.count, blocks = parts * a.tiles;
-    rc = check_grid(dev, what, std::max<u64>(blocks, static_cast<u64>(a.samples) * a.tiles * a.values.count) + a.channels);
+    const u64 parts = static_cast<u64>(a.samples) * a.parts.count;
+    a.channel_rows = static_cast<unsigned int>(parts);
+    if (plan.in_registers) {
+        const u64 together = std::max<u64>(1, kThreadsTogether / (static_cast<u64>(plan.threads) * a.tiles)), each = (parts + together - 1) / together;
+        a.channel_rows = static_cast<unsigned int>((parts + each - 1) / each);
+    }
+    const u64 blocks = static_cast<u64>(a.channel_rows) * a.tiles;
+    rc = check_grid(dev, what, plan.in_registers ? blocks : static_cast<u64>(a.samples) * a.tiles * std::max(a.parts.count, a.values.count) + a.channels, plan.threads);
     if (rc != CUSTOS_HIP_OK) return rc;
-    const size_t channel_bytes = parts * 2 * a.channels * sizeof(float), part_bytes = parts * a.groups * 2 * sizeof(float);
+    REQUIRE_DEV(dev);
+    const size_t channel_bytes = static_cast<u64>(a.channel_rows) * 2 * a.channels * sizeof(float), part_bytes = plan.in_registers ? 0 : parts * a.groups * 2 * sizeof(float);
     const size_t area_bytes = channel_bytes + part_bytes;
     uint64_t area = 0;
     rc = operator_workspace(dev, area_bytes, &area);

@@ -325,7 +325,7 @@ int32_t operator_workspace(custos_hip_device* dev, size_t bytes, uint64_t* addre
     return CUSTOS_HIP_OK;
 }
 
-int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* ops, size_t n, bool may_alias) {
+int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* ops, size_t n) {
     auto refuse = [&](int32_t code, const Operand& o, const char* why) {
         return set_error(dev, code, std::string(what) + ": " + o.name + " " + why);
     };
@@ -348,7 +348,7 @@ int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* 
             if (i == j || (o.written && j < i)) continue;
             if (!(w.ptr < o.end() && o.ptr < w.end())) continue;
             const bool one_pitch = w.pitch_bytes == o.pitch_bytes;
-            if (may_alias && !o.written && w.ptr == o.ptr && one_pitch && w.rows == o.rows && w.row_bytes == o.row_bytes) continue;
+            if (w.in_place && o.in_place && !o.written && w.ptr == o.ptr && one_pitch && w.rows == o.rows && w.row_bytes == o.row_bytes) continue;
             // slices of one wider tensor that share no element
             if (one_pitch && w.rows > 1 && o.rows > 1) {
                 const uint64_t pitch = w.pitch_bytes;
@@ -359,6 +359,11 @@ int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* 
         }
     }
     return CUSTOS_HIP_OK;
+}
+
+int32_t check_grid(custos_hip_device* dev, const char* what, uint64_t blocks, int threads) {
+    if (blocks < (1ull << 32) / static_cast<uint64_t>(threads)) return CUSTOS_HIP_OK;
+    return set_error(dev, CUSTOS_HIP_ERR_TOO_LARGE, std::string(what) + ": more than 2^32 threads in one launch");
 }
 
 }  // namespace custos_hip

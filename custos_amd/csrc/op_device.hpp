@@ -107,16 +107,10 @@ struct Bits {
     }
 };
 
-// Sum over the aligned groups of `WIDTH` lanes of a wavefront, in every lane (a fixed tree: results do not
-// depend on timing).
-template <int WIDTH>
+// Sum over a wavefront, in every lane (a fixed tree: results do not depend on timing).
 __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int step = WIDTH / 2; step > 0; step /= 2) v += __shfl_xor(v, step, 64);
-    return v;
-}
-__device__ __forceinline__ float lanes_sum_of(float v, int width) {
-    for (int step = width / 2; step > 0; step /= 2) v += __shfl_xor(v, step, 64);
+    for (int step = 32; step > 0; step /= 2) v += __shfl_xor(v, step, 64);
     return v;
 }
 __device__ __forceinline__ double lanes_sum_f64(double v) {

@@ -20,6 +20,7 @@
 // small difference.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "op_device.hpp"
 #include "runtime.hpp"
@@ -73,7 +74,7 @@ struct Running {
         float m = max;
 #pragma unroll
         for (int step = 32; step > 0; step /= 2) m = fmaxf(m, __shfl_xor(m, step, 64));
-        sum = lanes_sum<64>(sum * __builtin_amdgcn_exp2f((max - base(m)) * scale2));
+        sum = lanes_sum(sum * __builtin_amdgcn_exp2f((max - base(m)) * scale2));
         max = m;
     }
 };
@@ -399,10 +400,14 @@ int32_t custos_hip_token_logprob(custos_hip_device* dev, int32_t dtype, uint64_t
                       {"logp", logp, 1, rows * 4, 0, true, 4}};
     size_t n = 3;
     if (lse) ops[n++] = {"lse", lse, 1, rows * 4, 0, true, 4};
-    rc = check_operands(dev, what, ops, n, /*may_alias=*/false);
+    rc = check_operands(dev, what, ops, n);
+    if (rc != CUSTOS_HIP_OK) return rc;
+    const Kernel k = kernel_of<kLogprob>(dtype, static_cast<unsigned int>(vocab), false);
+    rc = check_grid(dev, what, rows, k.threads);
     if (rc != CUSTOS_HIP_OK) return rc;
     REQUIRE_DEV(dev);
-    RowArgs a{};
+    RowArgs a;
+    std::memset(&a, 0, sizeof a);  // (padding included: recordings compare the arguments of their launches byte by byte)
     a.logits = reinterpret_cast<const void*>(logits);
     a.labels = reinterpret_cast<const int*>(labels);
     a.logp = reinterpret_cast<float*>(logp);
@@ -413,7 +418,6 @@ int32_t custos_hip_token_logprob(custos_hip_device* dev, int32_t dtype, uint64_t
     a.scale2 = static_cast<float>(1.4426950408889634 / temperature);
     Access acc[4];
     for (size_t i = 0; i < n; i++) acc[i] = ops[i].access();
-    const Kernel k = kernel_of<kLogprob>(dtype, a.vocab, false);
     const OpArg arg{&a, sizeof a};
     return launch(dev, "custos_token_logprob", k.fn, rows, k.threads, &arg, 1, acc, n);
 }
@@ -435,9 +439,9 @@ int32_t custos_hip_policy_loss(custos_hip_device* dev, const custos_hip_policy_d
     Operand ops[9];
     size_t n = 0;
     if (rows > 0) {
-        if (logits_grad) ops[n++] = {"logits_grad", logits_grad, rows, desc->vocab * es, desc->grad_pitch * es, true, es};
+        if (logits_grad) ops[n++] = {"logits_grad", logits_grad, rows, desc->vocab * es, desc->grad_pitch * es, true, es, true};
         if (logp) ops[n++] = {"logp", logp, 1, rows * 4, 0, true, 4};
-        ops[n++] = {"logits", logits, rows, desc->vocab * es, desc->pitch * es, false, es};
+        ops[n++] = {"logits", logits, rows, desc->vocab * es, desc->pitch * es, false, es, true};
         ops[n++] = {"labels", labels, 1, rows * 4, 0, false, 4};
         ops[n++] = {"old_logp", old_logp, 1, rows * 4, 0, false, 4};
         ops[n++] = {"advantages", advantages, 1, rows * 4, 0, false, 4};
@@ -446,15 +450,15 @@ int32_t custos_hip_policy_loss(custos_hip_device* dev, const custos_hip_policy_d
     }
     const size_t without_totals = n;
     if (totals) ops[n++] = {"totals", totals, 1, 16, 0, true, 4};
-    rc = check_operands(dev, what, ops, n, /*may_alias=*/true);
+    rc = check_operands(dev, what, ops, n);
     if (rc != CUSTOS_HIP_OK) return rc;
-    // (only the gradient may take the place of what is read, and only of the logits: rows are worked on one by one)
-    for (uint64_t read : {labels, old_logp, ref_logp, advantages, weights})
-        if (read && rows > 0 && (read == logits_grad || read == logp || read == totals))
-            return set_error(dev, CUSTOS_HIP_ERR_BAD_OVERLAP, std::string(what) + ": an output overlaps an input");
+    const Kernel k = kernel_of<kPolicy>(desc->dtype, static_cast<unsigned int>(desc->vocab), 2 * rows * desc->vocab * es > kStreamBeyond);
+    rc = check_grid(dev, what, rows, k.threads);
+    if (rc != CUSTOS_HIP_OK) return rc;
     REQUIRE_DEV(dev);
     if (rows == 0) return totals ? custos_hip_clear(dev, totals, 16) : CUSTOS_HIP_OK;
-    RowArgs a{};
+    RowArgs a;
+    std::memset(&a, 0, sizeof a);  // (padding included: recordings compare the arguments of their launches byte by byte)
     a.logits = reinterpret_cast<const void*>(logits);
     a.labels = reinterpret_cast<const int*>(labels);
     a.old_logp = reinterpret_cast<const float*>(old_logp);
@@ -484,7 +488,6 @@ int32_t custos_hip_policy_loss(custos_hip_device* dev, const custos_hip_policy_d
         a.terms = reinterpret_cast<float4*>(area);
         acc[n_acc++] = {area, area + rows * sizeof(float4), true};
     }
-    const Kernel k = kernel_of<kPolicy>(desc->dtype, a.vocab, 2 * rows * desc->vocab * es > kStreamBeyond);
     const OpArg arg{&a, sizeof a};
     rc = launch(dev, "custos_policy_rows", k.fn, rows, k.threads, &arg, 1, acc, n_acc);
     if (rc != CUSTOS_HIP_OK || !totals) return rc;

@@ -427,14 +427,17 @@ struct Operand {
     uint64_t rows, row_bytes, pitch_bytes;
     bool written;
     size_t element;  // bytes its address has to be a multiple of
+    bool in_place = false;
     uint64_t end() const { return rows == 0 || row_bytes == 0 ? ptr : ptr + (rows - 1) * pitch_bytes + row_bytes; }
     Access access() const { return {ptr, end(), written}; }
 };
 // The checks every operator makes of its operands before it launches anything: no null or unaligned
 // address, no range that wraps, rows that do not overlap each other, and nothing written that another
-// operand covers -- except the same operand exactly (`may_alias`: the operator reads an element before it
-// writes it), and rows of one pitch that lie side by side (two slices of the same wider tensor).
-int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* ops, size_t n, bool may_alias);
+// operand covers -- except one and the same operand where both sides are `in_place` (the operator reads an element
+// before it writes it), and rows of one pitch that lie side by side (two slices of the same wider tensor).
+int32_t check_operands(custos_hip_device* dev, const char* what, const Operand* ops, size_t n);
+// A launch has fewer than 2^32 threads.
+int32_t check_grid(custos_hip_device* dev, const char* what, uint64_t blocks, int threads);
 
 // graph.cpp
 int32_t replay_graph(custos_hip_device* dev, custos_hip_graph* g);

@@ -450,7 +450,7 @@ enum custos_hip_activation {
  * even), scale = top * (1 / 127), and the code stands for code * scale, all in f32; so a finite value is
  * kept to within half a scale.  What is not finite gets code -128, which stands for NaN.  A block
  * whose top is below 2^-100 is kept as zeros.
- * `codes`: n bytes; `scales`: ceil(n / 128) f32.  n == 0: nothing is done.
+ * `codes`: n bytes; `scales`: ceil(n / 128) f32.  n == 0: nothing is done; n is at most 2^34.
  *
  * out[i] = f(x[i]) and the checkpoint of x in one pass; kernel of kind SAVE8.  out 0: only the checkpoint
  * is made.  out may be x exactly. */
@@ -497,8 +497,8 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device *dev, const custos_hip_
 
 /* Log-probabilities of chosen tokens: of every row of `vocab` logits (f32, f16 or bf16; `pitch` elements
  * from row to row), lse = log sum exp(z / T) and logp = z[label] / T - lse, f32 [rows] each; labels are
- * int32.  A negative label chooses nothing: its logp is 0, and without `lse` (0: not wanted) its row is
- * not read.  A label behind the vocabulary gives NaN.  Logits of -inf are tokens that cannot be chosen; a
+ * int32.  A negative label chooses nothing: its logp is 0, whatever the row holds; `lse` (0: not wanted)
+ * is that of the row.  A label behind the vocabulary gives NaN.  Logits of -inf are tokens that cannot be chosen; a
  * row of nothing else has no distribution: lse -inf, logp NaN.  A row of the type's lowest value
  * is a uniform one. */
 int32_t custos_hip_token_logprob(custos_hip_device *dev, int32_t dtype, uint64_t logits, uint64_t pitch, uint64_t labels,
@@ -520,7 +520,7 @@ typedef struct custos_hip_policy_desc {
  * rows of weight * (kl_coef * kl - min(r * advantage, clamp(r) * advantage)).  old_logp,
  * ref_logp (0: no KL term; kl_coef is 0 then), advantages and weights are f32 [rows]; weights hold the mask
  * and the normalisation (1 / tokens, or what a mean per sequence asks for).  A row with a negative
- * label or weight 0 is not read: its logp is 0, its gradient zeros, whatever the row holds.
+ * label or weight 0 does not count: its logp is 0, its gradient zeros, whatever the row holds.
  * `logits_grad` (0: not wanted; may be the logits exactly) is stored, not added to; `logp` (0: not
  * wanted) f32 [rows]; `totals` (0: not wanted) f32 [4]: the loss, and the weighted sums of kl, of the rows
  * whose clipped term is the smaller one, and of r.  No rows: the totals are zeros. */

@@ -178,6 +178,28 @@ def test_gradients_from_a_checkpoint(hip, n, p, c, groups, pad, dtype):
     check_gradients(case, gradients(hip, case, saved=saved), x=x)
 
 
+# more samples than workgroups: of 256 threads, and of 1024
+MANY = [(9000, 2, 24, 1), (20000, 1, 10, 5), (2100, 3, 1032, 1)]
+
+
+@pytest.mark.parametrize("n, p, c, groups", MANY)
+def test_many_samples(hip, n, p, c, groups):
+    case = Case(n, p, c, groups, "f32", seed=n)
+    check_forward(case, *forward(hip, case))
+    check_gradients(case, gradients(hip, case))
+    start = [np.ones(case.shape)] + [np.full(c, 3, np.float32) for _ in range(2)]
+    check_gradients(case, gradients(hip, case, overwrite=False, start=start), start=start)
+
+
+# few positions, so that a tile takes more channels than it needs to; groups that do not divide by two
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n, p, c, groups", [(600, 5, 90, 9), (300, 64, 80, 10), (1100, 1, 96, 12), (260, 17, 260, 65)])
+def test_wide_tiles(hip, n, p, c, groups, dtype):
+    case = Case(n, p, c, groups, dtype, seed=n)
+    check_forward(case, *forward(hip, case))
+    check_gradients(case, gradients(hip, case))
+
+
 @pytest.mark.parametrize("activation", ["none", "relu", "gelu"])
 @pytest.mark.parametrize("n, p, c, groups", [(2, 50, 48, 4), (1, 9000, 24, 3)])
 def test_gradients_are_added(hip, n, p, c, groups, activation):

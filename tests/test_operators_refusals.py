@@ -107,6 +107,38 @@ def test_group_norm_gradient_operands(over, code, text):
     refused(gn_grad(gn_desc(), **over), code, text)
 
 
+@pytest.mark.parametrize("eps", [1e-300, 1e-40, 1e39])
+def test_eps_is_a_normal_number_in_f32(eps):
+    refused(gn(gn_desc(eps=eps)), INVALID, "eps is positive")
+    refused(gn_grad(gn_desc(eps=eps)), INVALID, "eps is positive")
+
+
+def test_only_values_may_take_the_place_of_values():
+    """What one workgroup writes and another reads is no place for a result, however well the sizes fit."""
+    wide = dict(flags=1, channels=8, groups=2)
+    for over in (dict(gamma_grad=BASE + 0x60000), dict(beta_grad=BASE + 0x60000)):
+        refused(gn_grad(gn_desc(**wide), gamma=BASE + 0x60000, **over), OVERLAP, "overlaps gamma")
+    refused(gn_grad(gn_desc(**wide), beta=BASE + 0x60000, beta_grad=BASE + 0x60000), OVERLAP, "overlaps beta")
+    refused(gn_grad(gn_desc(**wide), gamma_grad=BASE + 0x10000), OVERLAP, "overlaps stats")
+    # one row: x, gamma and the statistics of four groups of two channels have as many bytes
+    row = dict(samples=1, positions=1, channels=8, groups=4)
+    refused(gn(gn_desc(**row), stats=BASE), OVERLAP, "overlaps x")
+    refused(gn(gn_desc(**row), stats=BASE + 0x10000), OVERLAP, "overlaps gamma")
+    refused(gn(gn_desc(**row), out=BASE + 0x10000), OVERLAP, "overlaps gamma")
+    refused(gn_grad(gn_desc(**row, flags=1), gamma=BASE + 0x30000), OVERLAP, "overlaps gamma")
+    refused(gn(gn_desc(**row), out=BASE), INVALID, "device handle is null")
+
+
+def test_launches_have_fewer_than_2_to_32_threads():
+    # (each in less than 2^32 bytes an operand or two)
+    refused(gn(gn_desc(samples=1 << 24, positions=1), out=1 << 40, stats=1 << 42), LARGE, "2^32 threads")
+    refused(gn_grad(gn_desc(samples=1 << 24, positions=1), x=1 << 46, stats=1 << 44, out_grad=1 << 42, x_grad=1 << 40, gamma_grad=1 << 30, beta_grad=1 << 31), INVALID, "device handle is null")
+    refused(logprob(rows=1 << 26, logits=1 << 40, labels=1 << 41, logp=1 << 42), LARGE, "2^32 threads")
+    refused(policy(dict(rows=1 << 26), logits=1 << 40, labels=1 << 41, old_logp=1 << 42, advantages=1 << 43, weights=1 << 44,
+                   logits_grad=1 << 45, logp=1 << 46, totals=1 << 47), LARGE, "2^32 threads")
+    refused(logprob(rows=(1 << 26) - 1, logits=1 << 40, labels=1 << 41, logp=1 << 42), INVALID, "device handle is null")
+
+
 def test_forward_takes_no_flags():
     refused(gn(gn_desc(flags=1)), INVALID, "no flags")
     refused(gn(None), INVALID, "description is null")
@@ -239,6 +271,8 @@ def test_rows_of_logits(over, code, text):
     ({}, dict(logp=BASE + 0x20000), OVERLAP, "overlaps"),
     ({}, dict(totals=BASE + 0x60000), OVERLAP, "overlaps"),
     ({}, dict(totals=BASE + 0x40000), OVERLAP, "overlaps"),
+    (dict(vocab=1, pitch=1, grad_pitch=1, rows=1), dict(logits_grad=BASE + 0x20000), OVERLAP, "overlaps old_logp"),
+    (dict(vocab=1, pitch=1, grad_pitch=1, rows=1), dict(logp=BASE), OVERLAP, "overlaps logits"),
 ])
 def test_policy_refusals(over, args, code, text):
     refused(policy(over, **args), code, text)
