@@ -61,6 +61,21 @@ struct HipDType<bf16_pernode> {
     static constexpr int32_t value = CUSTOS_HIP_BF16_PERNODE;
 };
 
+// Sizes of a group norm over [samples][positions][channels] without gaps, and its activation (CUSTOS_HIP_ACT_*).
+struct GroupNorm {
+    size_t samples, positions, channels, groups;
+    int32_t activation = CUSTOS_HIP_ACT_NONE;
+    double eps = 1e-5;
+};
+
+// What the clipped policy loss takes besides its operands.
+struct PolicyLoss {
+    double clip_low = 0.2, clip_high = 0.2;
+    double kl_coef = 0.0;
+    double temperature = 1.0;
+    double grad_scale = 1.0;
+};
+
 template <class Mods>
 class HIP : public Device<HIP<Mods>, Mods> {
    public:
@@ -127,6 +142,111 @@ class HIP : public Device<HIP<Mods>, Mods> {
         const std::string src = to_cl_source(f(Resolve<T>::with_marker("x")));
         custos_hip_kernel* k = compile(CUSTOS_HIP_KIND_UNARY_GRAD, HipDType<T>::value, src, {"x"});
         check(custos_hip_add_unary_grad(dev_, k, lhs.ptr(), lhs_grad.ptr(), out_grad.ptr(), lhs.len()));
+    }
+
+    // ---- operators of a training step (custos_hip.h) ----
+    //
+    // Like the `_impl` calls above they work on given buffers and can stand inside an `add_op`, where a
+    // recording picks them up.  Operands that may be left out are pointers: null is "not given".
+
+    // `f(x)` and x in 8 bits, in one pass; `codes` has x.len() elements, `scales` one per 128.
+    template <class T, class F>
+    void apply_fn_checkpoint8_impl(const Buffer<T, Self>& x, Buffer<T, Self>& out, Buffer<int8_t, Self>& codes,
+                                   Buffer<float, Self>& scales, F f) {
+        holds(out.len(), x.len());
+        holds8(codes, scales, x.len());
+        custos_hip_kernel* k =
+            compile(CUSTOS_HIP_KIND_SAVE8, HipDType<T>::value, to_cl_source(f(Resolve<T>::with_marker("x"))), {"x"});
+        check(custos_hip_checkpoint8_save(dev_, k, x.ptr(), given(&out), codes.ptr(), scales.ptr(), x.len()));
+    }
+    template <class T>
+    void checkpoint8_impl(const Buffer<T, Self>& x, Buffer<int8_t, Self>& codes, Buffer<float, Self>& scales) {
+        holds8(codes, scales, x.len());
+        custos_hip_kernel* k = compile(CUSTOS_HIP_KIND_SAVE8, HipDType<T>::value, "x", {"x"});
+        check(custos_hip_checkpoint8_save(dev_, k, x.ptr(), 0, codes.ptr(), scales.ptr(), x.len()));
+    }
+    // `f` of the values a checkpoint stands for
+    template <class T, class F>
+    void restore8_impl(const Buffer<int8_t, Self>& codes, const Buffer<float, Self>& scales, Buffer<T, Self>& out, F f) {
+        holds8(codes, scales, out.len());
+        custos_hip_kernel* k =
+            compile(CUSTOS_HIP_KIND_RESTORE8, HipDType<T>::value, to_cl_source(f(Resolve<T>::with_marker("x"))), {"x"});
+        check(custos_hip_checkpoint8_restore(dev_, k, codes.ptr(), scales.ptr(), out.ptr(), out.len()));
+    }
+    // `add_unary_grad_impl` with its input taken from a checkpoint
+    template <class T, class F>
+    void add_unary_grad8_impl(const Buffer<int8_t, Self>& codes, const Buffer<float, Self>& scales, Buffer<T, Self>& lhs_grad,
+                              const Buffer<T, Self>& out_grad, F f, bool overwrite = false) {
+        holds(lhs_grad.len(), out_grad.len());
+        holds8(codes, scales, out_grad.len());
+        custos_hip_kernel* k =
+            compile(CUSTOS_HIP_KIND_UNARY_GRAD8, HipDType<T>::value, to_cl_source(f(Resolve<T>::with_marker("x"))), {"x"});
+        check(custos_hip_add_unary_grad8(dev_, k, codes.ptr(), scales.ptr(), lhs_grad.ptr(), out_grad.ptr(), out_grad.len(),
+                                         overwrite ? CUSTOS_HIP_GRAD_OVERWRITE : 0));
+    }
+
+    // Group norm with an activation; `stats` has samples * groups * 2 elements.
+    template <class T, class P = T>
+    void group_norm_impl(const Buffer<T, Self>& x, const Buffer<P, Self>* gamma, const Buffer<P, Self>* beta,
+                         Buffer<T, Self>& out, Buffer<float, Self>& stats, const GroupNorm& norm) {
+        const custos_hip_group_norm_desc desc = norm_desc<T, P>(norm, 0);
+        const size_t len = product(product(norm.samples, norm.positions), norm.channels);
+        holds(x.len(), len);
+        holds(out.len(), len);
+        holds(stats.len(), product(product(norm.samples, norm.groups), 2));
+        for (const auto* p : {gamma, beta})
+            if (p) holds(p->len(), norm.channels);
+        check(custos_hip_group_norm(dev_, &desc, x.ptr(), norm.channels, given(gamma), given(beta), out.ptr(), norm.channels,
+                                    stats.ptr()));
+    }
+    // Its gradients, added or (`overwrite`) stored; the ones that are null are not computed.
+    template <class T, class P = T>
+    void add_group_norm_grad_impl(const Buffer<T, Self>& x, const Buffer<float, Self>& stats, const Buffer<P, Self>* gamma,
+                                  const Buffer<P, Self>* beta, const Buffer<T, Self>& out_grad, Buffer<T, Self>* x_grad,
+                                  Buffer<float, Self>* gamma_grad, Buffer<float, Self>* beta_grad, const GroupNorm& norm,
+                                  bool overwrite = false) {
+        holds(x.len(), out_grad.len());
+        norm_grad(x.ptr(), 0, 0, stats, gamma, beta, out_grad, x_grad, gamma_grad, beta_grad, norm, overwrite);
+    }
+    // the same with x as `checkpoint8_impl` left it
+    template <class T, class P = T>
+    void add_group_norm_grad8_impl(const Buffer<int8_t, Self>& codes, const Buffer<float, Self>& scales,
+                                   const Buffer<float, Self>& stats, const Buffer<P, Self>* gamma, const Buffer<P, Self>* beta,
+                                   const Buffer<T, Self>& out_grad, Buffer<T, Self>* x_grad, Buffer<float, Self>* gamma_grad,
+                                   Buffer<float, Self>* beta_grad, const GroupNorm& norm, bool overwrite = false) {
+        holds8(codes, scales, out_grad.len());
+        norm_grad(0, codes.ptr(), scales.ptr(), stats, gamma, beta, out_grad, x_grad, gamma_grad, beta_grad, norm, overwrite);
+    }
+
+    // Log-probabilities of chosen tokens over labels.len() rows of logits without gaps.
+    template <class T>
+    void token_logprob_impl(const Buffer<T, Self>& logits, const Buffer<int32_t, Self>& labels, Buffer<float, Self>& logp,
+                            Buffer<float, Self>* lse = nullptr, double temperature = 1.0) {
+        const size_t rows = labels.len(), vocab = row_len(logits, rows);
+        holds(logp.len(), rows);
+        if (lse) holds(lse->len(), rows);
+        check(custos_hip_token_logprob(dev_, HipDType<T>::value, logits.ptr(), vocab, labels.ptr(), rows, vocab, temperature,
+                                       logp.ptr(), given(lse)));
+    }
+
+    // Clipped policy loss with a KL term (with `ref_logp`) and its gradient over such rows.
+    template <class T>
+    void policy_loss_impl(const Buffer<T, Self>& logits, const Buffer<int32_t, Self>& labels, const Buffer<float, Self>& old_logp,
+                          const Buffer<float, Self>* ref_logp, const Buffer<float, Self>& advantages,
+                          const Buffer<float, Self>& weights, Buffer<T, Self>* logits_grad, Buffer<float, Self>* logp,
+                          Buffer<float, Self>* totals, const PolicyLoss& loss = {}) {
+        const size_t rows = labels.len(), vocab = row_len(logits, rows);
+        holds(old_logp.len(), rows);
+        holds(advantages.len(), rows);
+        holds(weights.len(), rows);
+        if (ref_logp) holds(ref_logp->len(), rows);
+        if (logits_grad) holds(logits_grad->len(), logits.len());
+        if (logp) holds(logp->len(), rows);
+        if (totals) holds(totals->len(), 4);
+        const custos_hip_policy_desc desc = {HipDType<T>::value, 0, rows, vocab, vocab, vocab, loss.temperature,
+                                             loss.clip_low, loss.clip_high, loss.kl_coef, loss.grad_scale};
+        check(custos_hip_policy_loss(dev_, &desc, logits.ptr(), labels.ptr(), old_logp.ptr(), given(ref_logp), advantages.ptr(),
+                                     weights.ptr(), given(logits_grad), given(logp), given(totals)));
     }
 
     // `UnaryFusing::unary_fuse_op` (src/devices/cuda/fusing.rs:8-50): one kernel
@@ -311,6 +431,53 @@ class HIP : public Device<HIP<Mods>, Mods> {
     }
 
    private:
+    static void holds(size_t len, size_t expected) {
+        if (len != expected) throw Error(DeviceError::ShapeLengthMismatch);
+    }
+    static size_t product(size_t a, size_t b) {
+        if (b && a > SIZE_MAX / b) throw Error(DeviceError::ShapeLengthMismatch);
+        return a * b;
+    }
+    static void holds8(const Buffer<int8_t, Self>& codes, const Buffer<float, Self>& scales, size_t len) {
+        holds(codes.len(), len);
+        holds(scales.len(), len / 128 + (len % 128 != 0));
+    }
+    template <class T>
+    static size_t row_len(const Buffer<T, Self>& logits, size_t rows) {
+        if (rows == 0) return 1;
+        holds(logits.len() % rows, 0);
+        return logits.len() / rows;
+    }
+    // the address of an operand that may be left out; one that is given but not allocated yet is an error,
+    // not an operand left out
+    template <class T>
+    static uint64_t given(const Buffer<T, Self>* buf) {
+        if (!buf) return 0;
+        if (!buf->has_data() && buf->len()) throw Error(DeviceError::InvalidLazyBuf);
+        return buf->ptr();
+    }
+    template <class T, class P>
+    static custos_hip_group_norm_desc norm_desc(const GroupNorm& norm, int32_t flags) {
+        return {HipDType<T>::value, HipDType<P>::value, norm.activation, flags, norm.samples, norm.positions, norm.channels,
+                norm.groups, norm.eps};
+    }
+    template <class T, class P>
+    void norm_grad(uint64_t x, uint64_t codes, uint64_t scales, const Buffer<float, Self>& stats, const Buffer<P, Self>* gamma,
+                   const Buffer<P, Self>* beta, const Buffer<T, Self>& out_grad, Buffer<T, Self>* x_grad,
+                   Buffer<float, Self>* gamma_grad, Buffer<float, Self>* beta_grad, const GroupNorm& norm, bool overwrite) {
+        const custos_hip_group_norm_desc desc = norm_desc<T, P>(norm, overwrite ? CUSTOS_HIP_GRAD_OVERWRITE : 0);
+        holds(out_grad.len(), product(product(norm.samples, norm.positions), norm.channels));
+        holds(stats.len(), product(product(norm.samples, norm.groups), 2));
+        if (x_grad) holds(x_grad->len(), out_grad.len());
+        for (const auto* p : {gamma, beta})
+            if (p) holds(p->len(), norm.channels);
+        for (const auto* p : {gamma_grad, beta_grad})
+            if (p) holds(p->len(), norm.channels);
+        check(custos_hip_add_group_norm_grad(dev_, &desc, x, norm.channels, codes, scales, stats.ptr(), given(gamma), given(beta),
+                                             out_grad.ptr(), norm.channels, given(x_grad), norm.channels, given(gamma_grad),
+                                             given(beta_grad)));
+    }
+
     // argument values laid out for the launch call: 8 bytes of storage each
     template <size_t N>
     struct KernelArgs {
