@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kBlock = 256;      // threads of the kernels that stream
 constexpr unsigned int kMaxTileGroups = 64;     // groups per tile of the kernels that hold a tile in registers
+constexpr int kAheadForward = 4, kAheadBackward = 2;  // rows a thread of the kernels that stream loads before it uses them
 constexpr int kMaxStreamGroups = 128;  // groups per tile of the kernels that stream
 
 enum Activation { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kBlock) custos_group_norm_parts(const GroupNor
                 q[j] = __builtin_fmaf(d, d, q[j]);
             }
         };
-        constexpr int kAhead = 4;
+        constexpr int kAhead = kAheadForward;
         u64 i = 0;
         for (; i + kAhead <= w.rows; i += kAhead) {
             Source<T, V, false> x[kAhead];
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(kBlock) custos_group_norm_values(const GroupNo
                     y.v[j] = from_f32<T>(act<ACT>(__builtin_fmaf(x.value(j), scale[j], shift[j])));
                 return y;
             };
-            constexpr int kAhead = 4;
+            constexpr int kAhead = kAheadForward;
             u64 i = 0;
             for (; i + kAhead <= w.rows; i += kAhead) {
                 Source<T, V, false> x[kAhead];
@@ -818,7 +819,7 @@ __global__ void __launch_bounds__(THREADS) custos_group_norm_grad_tile(const Gro
 template <class T, int V, bool SAVED, bool STREAM, class F>
 __device__ __forceinline__ void for_rows(const GroupNormArgs& a, const Stream<V>& w, unsigned int channel, F f) {
     const T* out_grad = static_cast<const T*>(a.out_grad) + channel;
-    constexpr int kAhead = 2;
+    constexpr int kAhead = kAheadBackward;
     u64 i = 0;
     for (; i + kAhead <= w.rows; i += kAhead) {
         Source<T, V, SAVED> x[kAhead];
@@ -995,9 +996,10 @@ struct Held {
 constexpr Held kForwardHeld[] = {{256, 4, ~0ull}, {256, 8, ~0ull}, {1024, 4, ~0ull}, {1024, 8, kStreamBeyond}, {1024, 16, kStreamBeyond}};
 constexpr Held kBackwardHeld[] = {{256, 4, ~0ull}, {512, 4, 32ull << 20}};
 
-// `accumulates`: the results are added to what is there, so no channel may be stored by two threads.
+// `accumulates`: the results are added to what is there, so no channel may be stored by two threads.  `rounds_each`: the
+// fewest rounds of rows of a workgroup of the first pass.
 template <size_t N>
-void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool accumulates, const Held (&choices)[N], Plan* plan) {
+void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool accumulates, const Held (&choices)[N], u64 rounds_each, Plan* plan) {
     GroupNormArgs& a = plan->a;
     a.positions = d.positions;
     a.samples = static_cast<unsigned int>(d.samples);
@@ -1062,8 +1064,11 @@ void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool
     a.step = static_cast<unsigned int>(std::max<u64>(1, kBlock / vecs));
     const u64 rounds = (a.positions + a.step - 1) / a.step, tiles = static_cast<u64>(a.samples) * a.tiles;
     plan->stream = moved > kStreamBeyond;
-    // what the chip holds at once, each with a few rounds of rows, and no more parts than are joined in passing
-    finish(std::min<u64>({std::max<u64>(1, 1024 / tiles), std::max<u64>(1, rounds / 4), std::max<u64>(1, 4096 / a.tile_groups)}),
+    // What the chip holds at once, each with a few rounds of rows, and no more parts than are joined in passing.  In the
+    // first pass two rounds of loads on the way to each thread: 8 rows forward, 4 backward (forward over 3x1961x330 f32
+    // 16.0, with 4 rows 17.3, with 2 21; over 20000x64 bf16 14.4, 15.5, 16.0; gradient over 4x1024x640 bf16 18.7, with 8
+    // rows 20.5), in the second 4 (with 8 the last two take 16.6 and 20.9).
+    finish(std::min<u64>({std::max<u64>(1, 1024 / tiles), std::max<u64>(1, rounds / rounds_each), std::max<u64>(1, 4096 / a.tile_groups)}),
            std::min<u64>(std::max<u64>(1, 2048 / tiles), std::max<u64>(1, rounds / 4)));
 }
 
@@ -1222,7 +1227,7 @@ int32_t custos_hip_group_norm(custos_hip_device* dev, const custos_hip_group_nor
     if (rc != CUSTOS_HIP_OK) return rc;
 
     Plan plan;
-    make_plan(*desc, es, 2 * rows * desc->channels * es, /*accumulates=*/false, kForwardHeld, &plan);
+    make_plan(*desc, es, 2 * rows * desc->channels * es, /*accumulates=*/false, kForwardHeld, 2 * kAheadForward, &plan);
     GroupNormArgs& a = plan.a;
     a.x = reinterpret_cast<const void*>(x);
     a.gamma = reinterpret_cast<const void*>(gamma);
@@ -1302,7 +1307,7 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device* dev, const custos_hip_
 
     Plan plan;
     make_plan(*desc, es, total * (saved ? 2 * es + 1 : 3 * es),
-              /*accumulates=*/!overwrite, kBackwardHeld, &plan);
+              /*accumulates=*/!overwrite, kBackwardHeld, 2 * kAheadBackward, &plan);
     GroupNormArgs& a = plan.a;
     a.x = reinterpret_cast<const void*>(x);
     a.codes = reinterpret_cast<const signed char*>(codes);
