@@ -479,7 +479,8 @@ typedef struct custos_hip_group_norm_desc {
  * beta), rounded once.  Pitches: elements from one position to the next (>= channels).  gamma or
  * beta 0: ones, zeros.  `stats` receives mean and 1 / sqrt(var + eps) as f32
  * [samples][groups][2], which the gradient takes.  out may be x exactly.  No samples or no positions:
- * nothing is done.  NaN and infinities in a group make that group's results NaN, as the formula does. */
+ * nothing is done.  NaN and infinities in a group make that group's results NaN, as the formula does; so do
+ * distances from the mean whose squares add up beyond f32 (about 1e18), or they leave 1 / sqrt at 0. */
 int32_t custos_hip_group_norm(custos_hip_device *dev, const custos_hip_group_norm_desc *desc, uint64_t x,
                               uint64_t x_pitch, uint64_t gamma, uint64_t beta, uint64_t out,
                               uint64_t out_pitch, uint64_t stats);
