@@ -1027,7 +1027,7 @@ void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool
         a.whole_groups = a.tile_groups == 1 || a.per_group % static_cast<unsigned int>(plan->vec) == 0;
         a.total_inverse = 1.0 / (static_cast<double>(a.positions) * a.per_group);
     };
-    // in registers, if a tile of whole groups of at least 64 bytes a row fits
+    // in registers, if a tile of whole groups fits whose rows are at least kTileRow bytes
     {
         unsigned int k = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>(kTileRow / elem), kMaxTileGroups);
         for (unsigned int wider = k + 1; wider <= std::min(a.groups, kMaxTileGroups); wider++) {
