@@ -903,6 +903,11 @@ int32_t check_desc(custos_hip_device* dev, const char* what, const custos_hip_gr
     return CUSTOS_HIP_OK;
 }
 
+// A plan outside what the kernels hold would write past their shared arrays.
+int32_t check_plan(custos_hip_device* dev, const char* what, const Plan& plan) {
+    if (fits(plan)) return CUSTOS_HIP_OK;
+    return set_error(dev, CUSTOS_HIP_ERR_TOO_LARGE, std::string(what) + ": no kernel holds a tile of these sizes");
+}
 
 template <class K>
 void* handle(K* kernel) {
@@ -1023,6 +1028,8 @@ int32_t custos_hip_group_norm(custos_hip_device* dev, const custos_hip_group_nor
     if (rc != CUSTOS_HIP_OK) return rc;
 
     Plan plan = forward_plan(*desc);
+    rc = check_plan(dev, "group norm", plan);
+    if (rc != CUSTOS_HIP_OK) return rc;
     GroupNormArgs& a = plan.a;
     a.x = reinterpret_cast<const void*>(x);
     a.gamma = reinterpret_cast<const void*>(gamma);
@@ -1101,6 +1108,8 @@ int32_t custos_hip_add_group_norm_grad(custos_hip_device* dev, const custos_hip_
     }
 
     Plan plan = gradient_plan(*desc, saved);
+    rc = check_plan(dev, what, plan);
+    if (rc != CUSTOS_HIP_OK) return rc;
     GroupNormArgs& a = plan.a;
     a.x = reinterpret_cast<const void*>(x);
     a.codes = reinterpret_cast<const signed char*>(codes);

@@ -105,12 +105,13 @@ inline Divisor divisor(unsigned int by) { return {by, by == 1 ? 0u : static_cast
 
 inline unsigned int magic_of(unsigned int d) { return d == 1 ? 0u : static_cast<unsigned int>((0x100000000ull + d - 1) / d); }
 
-// The smallest divisor of `groups` whose tile is at least `channels` wide (or all groups); if it is above `most`,
-// the largest one below.
-inline unsigned int tile_at_least(unsigned int groups, unsigned int per_group, unsigned int channels, unsigned int most) {
+// The smallest divisor of `groups` whose tile is at least `channels` wide (or all groups); if it is above `most`, or its
+// tile wider than `widest`, the largest one below (at the least one group, however wide).
+inline unsigned int tile_at_least(unsigned int groups, unsigned int per_group, unsigned int channels, unsigned int most, u64 widest) {
     unsigned int best = 1;
     for (unsigned int k = 1; k <= std::min(groups, most); k++)
         if (groups % k == 0) {
+            if (k > 1 && static_cast<u64>(k) * per_group > widest) break;
             best = k;
             if (static_cast<u64>(k) * per_group >= channels) break;
         }
@@ -162,7 +163,7 @@ void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool
     };
     // in registers, if a tile of whole groups fits whose rows are at least kTileRow bytes
     {
-        unsigned int k = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>(kTileRow / elem), kMaxTileGroups);
+        unsigned int k = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>(kTileRow / elem), kMaxTileGroups, ~0ull);
         for (unsigned int wider = k + 1; wider <= std::min(a.groups, kMaxTileGroups); wider++) {
             const u64 row = (static_cast<u64>(wider) * a.per_group + full - 1) / full;
             if (row > kBlock || a.positions > 4 * (kBlock / row) || static_cast<u64>(a.samples) * (a.groups / wider) < kTilesEnough) break;
@@ -188,7 +189,10 @@ void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool
             return;
         }
     }
-    a.tile_groups = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>((moved > kStreamBeyond ? 2 * kStreamRow : kStreamRow) / elem), kMaxStreamGroups);
+    // (of several groups only as wide as one vector a thread: the first pass keeps one column's sums, or one group's.
+    // With 17, 37, 41 groups and other primes the next divisor is all of them.)
+    a.tile_groups = tile_at_least(a.groups, a.per_group, static_cast<unsigned int>((moved > kStreamBeyond ? 2 * kStreamRow : kStreamRow) / elem), kMaxStreamGroups,
+                                  static_cast<u64>(kBlock) * full);
     const u64 width = static_cast<u64>(a.tile_groups) * a.per_group;
     plan->vec = static_cast<int>(width < full ? 1 : full);
     a.tiles = a.groups / a.tile_groups;
@@ -203,6 +207,16 @@ void make_plan(const custos_hip_group_norm_desc& d, size_t elem, u64 moved, bool
     // rows 20.5), in the second 4 (with 8 the last two take 16.6 and 20.9).
     finish(std::min<u64>({std::max<u64>(1, 1024 / tiles), std::max<u64>(1, rounds / rounds_each), std::max<u64>(1, 4096 / a.tile_groups)}),
            std::min<u64>(std::max<u64>(1, 2048 / tiles), std::max<u64>(1, rounds / 4)));
+}
+
+// What the kernels take for granted: their shared arrays hold a row of every thread, one group per tile or one column per
+// thread, and the groups of a tile.
+inline bool fits(const Plan& plan) {
+    const GroupNormArgs& a = plan.a;
+    if (plan.in_registers)
+        return a.tile_groups <= kMaxTileGroups && static_cast<u64>(a.step) * a.vecs <= static_cast<u64>(plan.threads) &&
+               a.positions <= static_cast<u64>(a.step) * static_cast<u64>(plan.held);
+    return a.tile_groups <= static_cast<unsigned int>(kMaxStreamGroups) && (a.tile_groups == 1 || static_cast<u64>(a.step) * a.vecs <= static_cast<u64>(kBlock));
 }
 
 // The second pass of a streaming plan whose rows are no whole vectors and whose results are added to, or take the place
