@@ -148,7 +148,9 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, u64 row, const RowI
     const double behind = a.ref_logp ? static_cast<double>(in.ref_logp) - logp : 0.0;
     // exp - 1 of both differences at once, in two lanes
     const double em1 = expm1(lane == 0 ? moved : behind);
-    const double ratio = __shfl(em1, 0, 64) + 1.0, behind_em1 = __shfl(em1, 1, 64);
+    const double behind_em1 = __shfl(em1, 1, 64);
+    double ratio = __shfl(em1, 0, 64) + 1.0;
+    if (ratio < 0.5) ratio = exp(moved);  // (the sum cancels: a ratio of e^-30 would have four digits, one of e^-37 none)
     const double kl = behind_em1 - behind;
     const double plain = ratio * advantage;
     const double clipped = fmin(fmax(ratio, 1.0 - a.clip_low), 1.0 + a.clip_high) * advantage;
