@@ -156,10 +156,11 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, u64 row, const RowI
     const double clipped = fmin(fmax(ratio, 1.0 - a.clip_low), 1.0 + a.clip_high) * advantage;
     const bool inside = !(plain > clipped);  // (a NaN stays one)
     const double value = inside ? plain : clipped;
+    const bool counts = a.kl_coef != 0.0;  // (a KL term that is only watched may be infinite: 0 times it is no number)
     if (lane == 0 && a.terms)
-        a.terms[row] = make_float4(static_cast<float>(weight * (a.kl_coef * kl - value)), static_cast<float>(weight * kl),
+        a.terms[row] = make_float4(static_cast<float>(weight * (counts ? a.kl_coef * kl - value : -value)), static_cast<float>(weight * kl),
                                    inside ? 0.0f : in.weight, static_cast<float>(weight * ratio));
-    const double slope = weight * ((inside ? -plain : 0.0) - a.kl_coef * behind_em1) * a.grad_factor;
+    const double slope = weight * ((inside ? -plain : 0.0) - (counts ? a.kl_coef * behind_em1 : 0.0)) * a.grad_factor;
     out->base = Running::base(run.max);
     out->slope = static_cast<float>(slope);
     out->factor = static_cast<float>(-slope / static_cast<double>(run.sum));

@@ -519,9 +519,11 @@ typedef struct custos_hip_policy_desc {
 /* Clipped policy loss with a KL term over chosen tokens, and its gradient to the logits.  With logp as
  * above, r = exp(logp - old_logp), d = ref_logp - logp and kl = exp(d) - 1 - d, the loss is the sum over
  * rows of weight * (kl_coef * kl - min(r * advantage, clamp(r) * advantage)).  old_logp,
- * ref_logp (0: no KL term; kl_coef is 0 then), advantages and weights are f32 [rows]; weights hold the mask
- * and the normalisation (1 / tokens, or what a mean per sequence asks for).  A row with a negative
- * label or weight 0 does not count: its logp is 0, its gradient zeros, whatever the row holds.
+ * ref_logp (0: no KL term; kl_coef is 0 then), advantages and weights are f32 [rows].  With ref_logp and
+ * kl_coef 0 the KL term is only summed for the totals: it moves neither loss nor gradient, even where it is
+ * not finite.  The weights hold the mask and the normalisation (1 / tokens, or what a mean per sequence asks
+ * for).  A row with a negative label or weight 0 does not count: its logp is 0, its gradient zeros, whatever
+ * the row holds.
  * `logits_grad` (0: not wanted; may be the logits exactly) is stored, not added to; `logp` (0: not
  * wanted) f32 [rows]; `totals` (0: not wanted) f32 [4]: the loss, and the weighted sums of kl, of the rows
  * whose clipped term is the smaller one, and of r.  No rows: the totals are zeros. */

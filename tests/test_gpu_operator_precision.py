@@ -39,3 +39,31 @@ def test_the_gradient_of_small_ratios(hip, vocab):
         got = totals.read().astype(np.float64)
         assert abs(got[3] - want_ratio) <= refs.STEP * want_ratio, (moved[r], got[3], want_ratio)
         assert abs(got[0] + want_ratio * a32[r]) <= refs.STEP * want_ratio * a32[r], moved[r]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [5, 9000])
+def test_a_kl_term_without_weight_moves_nothing(hip, vocab, dtype):
+    """ref_logp given to watch the KL term, kl_coef 0: loss and gradient are those of the call without it, also where the KL
+    term is beyond its type."""
+    rows = 4
+    rng = np.random.default_rng(vocab)
+    z = rng.normal(size=(rows, vocab))
+    labels = rng.integers(0, vocab, rows).astype(np.int32)
+    z[1, labels[1]] = -np.inf  # the chosen token is masked: its log-probability is -inf
+    logp = refs.token_logprob(z, labels, 1.0)[0]
+    ref = np.where(np.isfinite(logp), logp + 0.3, -1.0)
+    ref[2] = 800.0             # exp(d) beyond f64
+    old, advantages, weights = buffers(hip, np.where(np.isfinite(logp), logp - 0.1, -2.0), np.ones(rows), np.full(rows, 0.25))
+    logits, ids = hip.buffer(refs.store(z, dtype).reshape(-1), dtype), hip.buffer(labels, "i32")
+    plain = hip.policy_loss(logits, ids, old, advantages, weights, (rows, vocab))
+    watched = hip.policy_loss(logits, ids, old, advantages, weights, (rows, vocab), ref_logp=hip.buffer(ref.astype(np.float32)), kl_coef=0.0)
+    p, w = plain[0].read(), watched[0].read()
+    assert np.isfinite(p).all() and w[0] == p[0] and np.array_equal(w[2:], p[2:])
+    g = refs.load(watched[2].read(), dtype)
+    assert np.isfinite(g).all() and np.array_equal(g, refs.load(plain[2].read(), dtype))
+    # the KL total is still told (rows whose KL term is finite)
+    some = hip.buffer(np.array([0.25, 0, 0, 0.25], np.float32))
+    kl = hip.policy_loss(logits, ids, old, advantages, some, (rows, vocab), ref_logp=hip.buffer(ref.astype(np.float32)), kl_coef=0.0)[0].read()[1]
+    want = 0.5 * (np.expm1(0.3) - 0.3)  # (d is off by f32's rounding of ref, of magnitude log(vocab) + 3, and for bf16 by that of the logits)
+    assert abs(kl - want) < (1e-4 if dtype == "f32" else 0.1)
