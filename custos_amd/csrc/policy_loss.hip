@@ -44,8 +44,8 @@ struct RowArgs {
     float4* terms;          // policy: [rows], the four totals' parts; null: not wanted
     u64 pitch, grad_pitch;
     unsigned int vocab;
-    float inv_t, scale2;    // 1 / T, log2(e) / T
-    double clip_low, clip_high, kl_coef, grad_factor;
+    float scale2;           // log2(e) / T
+    double inv_t, clip_low, clip_high, kl_coef, grad_factor;  // inv_t: 1 / T
 };
 
 enum Mode { kLogprob = 0, kPolicy = 1 };
@@ -135,12 +135,11 @@ template <int MODE>
 __device__ __forceinline__ void finish_row(const RowArgs& a, u64 row, const RowInputs& in, const Running& run, RowGradient* out) {
     const unsigned int lane = threadIdx.x % 64;
     const double log_sum = log(static_cast<double>(run.sum));
-    const double inv_t = static_cast<double>(a.inv_t);
     const bool chosen = in.label >= 0;
-    const double logp = (static_cast<double>(in.z_label) - static_cast<double>(run.max)) * inv_t - log_sum;
+    const double logp = (static_cast<double>(in.z_label) - static_cast<double>(run.max)) * a.inv_t - log_sum;
     if (lane == 0 && a.logp) a.logp[row] = chosen ? static_cast<float>(logp) : 0.0f;
     if (MODE == kLogprob) {
-        if (lane == 0 && a.lse) a.lse[row] = static_cast<float>(static_cast<double>(run.max) * inv_t + log_sum);
+        if (lane == 0 && a.lse) a.lse[row] = static_cast<float>(static_cast<double>(run.max) * a.inv_t + log_sum);
         return;
     }
     const double weight = in.weight, advantage = in.advantage;
@@ -420,7 +419,7 @@ int32_t custos_hip_token_logprob(custos_hip_device* dev, int32_t dtype, uint64_t
     a.lse = reinterpret_cast<float*>(lse);
     a.pitch = pitch;
     a.vocab = static_cast<unsigned int>(vocab);
-    a.inv_t = static_cast<float>(1.0 / temperature);
+    a.inv_t = 1.0 / temperature;
     a.scale2 = static_cast<float>(1.4426950408889634 / temperature);
     Access acc[4];
     for (size_t i = 0; i < n; i++) acc[i] = ops[i].access();
@@ -476,7 +475,7 @@ int32_t custos_hip_policy_loss(custos_hip_device* dev, const custos_hip_policy_d
     a.pitch = desc->pitch;
     a.grad_pitch = desc->grad_pitch;
     a.vocab = static_cast<unsigned int>(desc->vocab);
-    a.inv_t = static_cast<float>(1.0 / desc->temperature);
+    a.inv_t = 1.0 / desc->temperature;
     a.scale2 = static_cast<float>(1.4426950408889634 / desc->temperature);
     a.clip_low = desc->clip_low;
     a.clip_high = desc->clip_high;

@@ -67,3 +67,19 @@ def test_a_kl_term_without_weight_moves_nothing(hip, vocab, dtype):
     kl = hip.policy_loss(logits, ids, old, advantages, some, (rows, vocab), ref_logp=hip.buffer(ref.astype(np.float32)), kl_coef=0.0)[0].read()[1]
     want = 0.5 * (np.expm1(0.3) - 0.3)  # (d is off by f32's rounding of ref, of magnitude log(vocab) + 3, and for bf16 by that of the logits)
     assert abs(kl - want) < (1e-4 if dtype == "f32" else 0.1)
+
+
+@pytest.mark.parametrize("temperature", [0.7, 1.3, 0.1, 3.0])
+def test_temperatures_that_f32_does_not_hold(hip, temperature):
+    """Two choices so far apart that the sum is exactly one: logp and lse are quotients, rounded once."""
+    rng = np.random.default_rng(4)
+    rows = 300
+    z = np.zeros((rows, 2), np.float32)
+    z[:, 0] = rng.uniform(-2000, 2000, rows)
+    z[:, 1] = z[:, 0] - rng.uniform(500, 5000, rows).astype(np.float32)
+    labels = np.ones(rows, np.int32)
+    lse = hip.alloc(rows)
+    got = hip.token_logprob(hip.buffer(z.reshape(-1)), hip.buffer(labels, "i32"), (rows, 2), temperature=temperature, lse=lse).read()
+    z64 = z.astype(np.float64)
+    refs.assert_close(got, (z64[:, 1] - z64[:, 0]) / temperature, F32 * np.abs(z64[:, 1] - z64[:, 0]) / temperature * (1 + 1e-6), "logp")
+    refs.assert_close(lse.read(), z64[:, 0] / temperature, F32 * np.abs(z64[:, 0]) / temperature * (1 + 1e-6), "lse")
