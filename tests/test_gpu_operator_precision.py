@@ -83,3 +83,22 @@ def test_temperatures_that_f32_does_not_hold(hip, temperature):
     z64 = z.astype(np.float64)
     refs.assert_close(got, (z64[:, 1] - z64[:, 0]) / temperature, F32 * np.abs(z64[:, 1] - z64[:, 0]) / temperature * (1 + 1e-6), "logp")
     refs.assert_close(lse.read(), z64[:, 0] / temperature, F32 * np.abs(z64[:, 0]) / temperature * (1 + 1e-6), "lse")
+
+
+@pytest.mark.parametrize("p, c", [(262144, 127), (65536, 127)])
+def test_an_outlier_at_the_first_position_does_not_cost_the_deviation(hip, p, c):
+    """One value in a group that the others lie up to 3000 deviations away from, where a thread meets it first."""
+    rng = np.random.default_rng(p)
+    x = rng.normal(size=(1, p, c)).astype(np.float32)
+    x[0, 0] = np.geomspace(30, 3000, c)
+    out, stats = hip.group_norm(hip.buffer(x.reshape(-1)), None, None, (1, p, c), c)
+    x64 = x[0].astype(np.float64)
+    mean, var = x64.mean(0), x64.var(0)
+    rstd = 1 / np.sqrt(var + 1e-5)
+    got = stats.read().astype(np.float64).reshape(c, 2)
+    # at most 1024 squares are added one after the other, and 64 operations follow; half of that in the root
+    chain = (1024 + 64) * F32
+    refs.assert_close(got[:, 0], mean, chain * (np.abs(x64).mean(0)), "mean")
+    refs.assert_close(got[:, 1], rstd, (chain / 2 + 2 * F32) * rstd, "rstd")
+    z = (x64 - mean) * rstd
+    refs.assert_close(out.read().reshape(p, c), z, 4 * chain * (1 + np.abs(z)), "out")
