@@ -226,6 +226,18 @@ __device__ __forceinline__ float block_sum(float v, float* wave_sums) {
     return total;
 }
 
+template <int THREADS>
+__device__ __forceinline__ double block_sum_f64(double v, double* wave_sums) {
+    v = lanes_sum_f64(v);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) wave_sums[threadIdx.x / 64] = v;
+    __syncthreads();
+    double total = 0.0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) total += wave_sums[w];
+    return total;
+}
+
 // The rows of a tile that one workgroup of a streaming kernel works on, and its threads' shares.  The workgroups of a
 // sample take turns, `step` rows at a time, so that those that run together read neighbouring memory (each on a
 // stretch of its own, at equal distances, they would meet in the same memory channels).
@@ -360,14 +372,22 @@ __global__ void __launch_bounds__(THREADS) custos_group_norm_tile(const GroupNor
 template <class T, int V>
 __global__ void __launch_bounds__(kBlock) custos_group_norm_parts(const GroupNormArgs a) {
     __shared__ float2 table[kBlock * V];
-    __shared__ float wave_sums[kBlock / 64];
+    __shared__ double wave_sums[kBlock / 64];
     __shared__ float2 group[kMaxStreamGroups];
     const unsigned int t = threadIdx.x;
     const Stream<V> w(a, a.parts, blockIdx.x);
     float2* out = reinterpret_cast<float2*>(a.group_parts) + static_cast<u64>(w.part) * a.groups + w.tile * a.tile_groups;
     const float rows = static_cast<float>(w.rows);
-    // of the thread, over all its columns (one group per tile), or of its column
-    float all = 0.0f, all_mean = 0.0f, all_m2 = 0.0f;
+    // One group per tile: sums over all columns of the thread, in f64 and about a value of the group that all threads of
+    // the workgroup read, so that no large numbers cancel (as merge_groups has it for tiles of several).
+    float base = 0.0f;
+    if (a.tile_groups == 1) {
+        Source<T, 1, false> x;
+        x.load(a, w.first - w.r0, w.c0);
+        base = x.value(0);
+    }
+    double all = 0.0, all_squares = 0.0;
+    const double per_row = w.rows > 0 ? 1.0 / static_cast<double>(w.rows) : 0.0;
     float mean[V], m2[V];
     Column c = column_of<V>(a, w.col0);
     for (unsigned int col = w.col0; col < w.vecs && w.active(); col += kBlock) {
@@ -430,27 +450,27 @@ __global__ void __launch_bounds__(kBlock) custos_group_norm_parts(const GroupNor
             }
         }
         if (a.tile_groups == 1 && w.rows > 0) {
-            // the column's channels are one group's: count, mean and squared distances of the thread
-            const float valid = static_cast<float>(V - c.dup), count = rows * valid;
-            float m = 0.0f, d2 = 0.0f;
+            double d1 = 0.0, d2 = 0.0;
+            float squares = 0.0f;
 #pragma unroll
-            for (int j = 0; j < V; j++) m += j >= c.dup ? mean[j] : 0.0f;
-            m /= valid;
-#pragma unroll
-            for (int j = 0; j < V; j++)
-                if (j >= c.dup) d2 += m2[j] + rows * (mean[j] - m) * (mean[j] - m);
-            const float both = all + count, delta = m - all_mean;
-            all_m2 += d2 + delta * delta * (all * (count / both));
-            all_mean += delta * (count / both);
-            all = both;
+            for (int j = 0; j < V; j++) {
+                const bool mine = j >= c.dup;
+                const double d = mine ? __builtin_fma(s[j], per_row, static_cast<double>(shift[j]) - base) : 0.0;
+                d1 += d;
+                d2 = __builtin_fma(d, d, d2);
+                squares += mine ? m2[j] : 0.0f;
+            }
+            all = __builtin_fma(rows, d1, all);
+            all_squares = __builtin_fma(rows, d2, all_squares + squares);
         }
     }
     const unsigned int split = w.part - w.n * a.parts.count;
     const float total_inverse = 1.0f / (static_cast<float>(part_rows(a, split)) * static_cast<float>(a.per_group));
     if (a.tile_groups == 1) {
-        const float m = block_sum<kBlock>(all * all_mean, wave_sums) * total_inverse;
-        const float d2 = block_sum<kBlock>(all_m2 + all * (all_mean - m) * (all_mean - m), wave_sums);
-        if (t == 0) *out = make_float2(m, d2);
+        all = block_sum_f64<kBlock>(all, wave_sums);
+        all_squares = block_sum_f64<kBlock>(all_squares, wave_sums);
+        const double m = all / (static_cast<double>(part_rows(a, split)) * a.per_group);
+        if (t == 0) *out = make_float2(static_cast<float>(base + m), static_cast<float>(not_negative(all_squares - all * m)));
         return;
     }
     if (w.active()) {

@@ -102,3 +102,25 @@ def test_an_outlier_at_the_first_position_does_not_cost_the_deviation(hip, p, c)
     refs.assert_close(got[:, 1], rstd, (chain / 2 + 2 * F32) * rstd, "rstd")
     z = (x64 - mean) * rstd
     refs.assert_close(out.read().reshape(p, c), z, 4 * chain * (1 + np.abs(z)), "out")
+
+
+@pytest.mark.parametrize("offset", [300.0, 1000.0, 20011.0])
+@pytest.mark.parametrize("p, c", [(4100, 97), (40, 9001), (700, 331), (3, 70000), (20000, 129)])
+def test_the_mean_of_one_wide_group_far_from_zero(hip, p, c, offset):
+    rng = np.random.default_rng(int(offset) + c)
+    x = (rng.normal(size=(1, p, c)) + offset).astype(np.float32)
+    _, stats = hip.group_norm(hip.buffer(x.reshape(-1)), None, None, (1, p, c), 1)
+    _, mean, rstd, _ = refs.group_norm(x.astype(np.float64), np.ones(c), np.zeros(c), 1, "none", 1e-5)
+    got = stats.read().astype(np.float64)
+    # the mean of a part and that of the group are each rounded once; everything else is a distance from a value (of size 5 at most)
+    assert abs(got[0] - mean[0, 0]) <= 2 * F32 * abs(mean[0, 0]) * 1.001 + refs.STEP * 5, (got[0], mean[0, 0])
+    assert abs(got[1] - rstd[0, 0]) <= refs.STEP * rstd[0, 0], (got[1], rstd[0, 0])
+
+
+@pytest.mark.parametrize("value", [1000.1, -3.3e5, 1e-3])
+@pytest.mark.parametrize("p, c", [(4100, 97), (40, 9001), (700, 331), (3, 70000)])
+def test_one_wide_group_of_equal_values_has_exactly_their_mean(hip, p, c, value):
+    _, stats = hip.group_norm(hip.buffer(np.full(p * c, value)), None, None, (1, p, c), 1)
+    assert stats.read()[0] == np.float32(value)
+    rstd = 1 / np.sqrt(np.float64(np.float32(1e-5)))
+    assert abs(stats.read()[1] - rstd) <= 4 * F32 * rstd  # (a root and a quotient)
