@@ -10,7 +10,8 @@
 //
 // Both directions move every element of their operands once and compute a dozen or two operations on it, so
 // they are bound by memory, and what counts is how often x is read.  A group's values are scattered (Cg
-// neighbours out of every position), so a workgroup takes whole rows of a tile of neighbouring groups.
+// neighbours out of every position), so a workgroup takes whole rows of a tile of neighbouring groups (which tile, and
+// how the rows are dealt out: group_norm_plan.hpp).
 //
 // Statistics are held in f32 and never as a difference of large sums: a mean, and the sum of squared
 // distances from it (merged as count, mean and that sum), in f64 where the parts of a group are joined.
